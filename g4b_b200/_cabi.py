@@ -119,6 +119,27 @@ class G4bAdvanceArgs(ctypes.Structure):
     ]
 
 
+class G4bRopePackedArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", G4bTensor), ("k", G4bTensor), ("v", G4bTensor), ("q_out", G4bTensor), ("rope_freqs", G4bTensor),
+        ("positions", G4bTensor), ("pair_axis", G4bTensor), ("q_starts", G4bTensor), ("time_dim_sizes", G4bTensor),
+        ("q_norm_w", G4bTensor), ("k_norm_w", G4bTensor), ("k_pool", G4bTensor), ("v_pool", G4bTensor),
+        ("block_tables", G4bTensor), ("rmsnorm_eps", ctypes.c_float), ("page_size", ctypes.c_int32),
+        ("norm_qk", ctypes.c_int32), ("norm_v", ctypes.c_int32),
+    ]
+
+
+class G4bPagePool(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("page_bytes", ctypes.c_int64)]
+
+
+class G4bPageCopyArgs(ctypes.Structure):
+    _fields_ = [
+        ("pools", ctypes.POINTER(G4bPagePool)), ("num_pages", ctypes.c_int64), ("src_pages", G4bTensor),
+        ("dst_pages", G4bTensor), ("num_pools", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 # every symbol include/g4b_attn.h declares: name -> (restype, argtypes)
 EXPORTS = {
     "g4b_flash_attention": (ctypes.c_int, [ctypes.POINTER(G4bAttnArgs), ctypes.c_void_p]),
@@ -137,6 +158,8 @@ EXPORTS = {
     "g4b_kv_append": (ctypes.c_int, [ctypes.POINTER(G4bAppendArgs), ctypes.c_void_p]),
     "g4b_rope_norm_append": (ctypes.c_int, [ctypes.POINTER(G4bRopeAppendArgs), ctypes.c_void_p]),
     "g4b_advance_decode_state": (ctypes.c_int, [ctypes.POINTER(G4bAdvanceArgs), ctypes.c_void_p]),
+    "g4b_rope_norm_append_packed": (ctypes.c_int, [ctypes.POINTER(G4bRopePackedArgs), ctypes.c_void_p]),
+    "g4b_page_copy": (ctypes.c_int, [ctypes.POINTER(G4bPageCopyArgs), ctypes.c_void_p]),
     "g4b_last_error_string": (ctypes.c_char_p, []),
     "g4b_abi_version": (ctypes.c_int, []),
     "g4b_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32)]),

@@ -73,6 +73,8 @@ int launch_decode_stream(const G4bAttnArgs& a, int num_splits, const G4bDecodeSt
 int launch_kv_append_fp8(const G4bFp8AppendArgs& a, cudaStream_t st);
 int launch_kv_dequant_fp8(const G4bFp8DequantArgs& a, cudaStream_t st);
 int launch_prefill(const G4bAttnArgs& a, cudaStream_t st);
+int launch_rope_norm_append_packed(const G4bRopePackedArgs& a, cudaStream_t st);
+int launch_page_copy(const G4bPageCopyArgs& a, cudaStream_t st);
 
 // ---------------------------------------------------------------------------------------
 // device: scalar conversions

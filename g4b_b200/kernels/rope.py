@@ -99,3 +99,61 @@ def rope_norm_append(
     a.norm_v = 1 if norm_v else 0
     _launch(a, stream)
     return None
+
+
+def rope_norm_append_packed(
+    q,
+    k,
+    v,
+    rope_freqs,
+    positions,
+    q_starts,
+    time_dim_sizes,
+    k_pool,
+    v_pool,
+    rmsnorm_eps: float,
+    *,
+    block_tables,
+    page_size: int = 16,
+    pair_axis=None,
+    q_out=None,
+    q_rmsnorm_w=None,
+    k_rmsnorm_w=None,
+    norm_qk: bool = True,
+    norm_v: bool = True,
+    stream=None,
+):
+    """``rope_norm_append`` for packed rows (``g4b_rope_norm_append_packed``): ``q [N,H,D]`` and
+    ``k, v [N,G,D]`` hold the new rows of several slots behind one another, slot b's at
+    ``[q_starts[b], q_starts[b+1])``, the last of its ``time_dim_sizes[b]`` tokens.
+
+    ``positions [axes,N]`` (or ``[N]``, or None: the row's place in the cache) are the rotary positions;
+    pair ``(i, i + D/2)`` of row n turns by ``positions[pair_axis[i], n] * rope_freqs[i]``, so that
+    ``pair_axis [D/2]`` (uint8) deals the pairs to time, height and width in sections or in turn.
+    The rotated q goes to ``q_out`` (any float dtype) or back into ``q``; k and v go to their slots'
+    pages.  No counterpart in the reference."""
+    a = _cabi.G4bRopePackedArgs()
+    a.q = _cabi.as_tensor(q)
+    a.k = _cabi.as_tensor(k)
+    a.v = _cabi.as_tensor(v)
+    a.q_out = _cabi.as_tensor(q_out)
+    a.rope_freqs = _cabi.as_tensor(rope_freqs)
+    a.positions = _cabi.as_tensor(positions)
+    if positions is not None and a.positions.ndim == 1:
+        a.positions.ndim = 2
+        a.positions.shape[1], a.positions.stride[1] = a.positions.shape[0], a.positions.stride[0]
+        a.positions.shape[0], a.positions.stride[0] = 1, 0
+    a.pair_axis = _cabi.as_tensor(pair_axis)
+    a.q_starts = _cabi.as_tensor(q_starts)
+    a.time_dim_sizes = _cabi.as_tensor(time_dim_sizes)
+    a.q_norm_w = _cabi.as_tensor(q_rmsnorm_w)
+    a.k_norm_w = _cabi.as_tensor(k_rmsnorm_w)
+    a.k_pool = _cabi.as_tensor(k_pool)
+    a.v_pool = _cabi.as_tensor(v_pool)
+    a.block_tables = _cabi.as_tensor(block_tables)
+    a.rmsnorm_eps = float(rmsnorm_eps)
+    a.page_size = int(page_size)
+    a.norm_qk = 1 if norm_qk else 0
+    a.norm_v = 1 if norm_v else 0
+    _cabi.check(_cabi.load().g4b_rope_norm_append_packed(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
+    return None

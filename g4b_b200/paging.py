@@ -73,6 +73,14 @@ class PageAllocator:
             if self._refs[p] == 0:
                 self._free.append(p)
 
+    def move(self, src, dst) -> None:
+        """Page src[i] is called dst[i] from now on; every dst must be free."""
+        if len(set(map(int, dst))) != len(dst) or any(self._refs[p] != 0 for p in dst) or any(self._refs[p] <= 0 for p in src):
+            raise RuntimeError("pages move from allocated ids to free ones")
+        self._refs[dst] = self._refs[src]
+        self._refs[src] = 0
+        self._free = [int(p) for p in np.flatnonzero(self._refs == 0)[::-1]]   # pop() hands out the lowest first
+
 
 @dataclass
 class _Slot:
@@ -101,6 +109,7 @@ class PagedKVManager:
         self.cache_offsets = np.zeros(self.max_batch, dtype=np.int32)
         self.time_dim_sizes = np.zeros(self.max_batch, dtype=np.int32)
         self.user_phase = np.zeros(self.max_batch, dtype=np.uint8)
+        self.q_starts = np.zeros(self.max_batch + 1, dtype=np.int32)   # packed steps: slot b owns rows [q_starts[b], q_starts[b+1])
         self.tables_dirty = True
         self._tick = 0
         self._device = None
@@ -159,6 +168,71 @@ class PagedKVManager:
         s.tokens = s.tokens[: s.filled]
         self._tick += 1
         s.retired_at = self._tick
+
+    def free(self, slot: int) -> None:
+        """The slot's request ended and its pages go back to the pool at once, without staying
+        behind as a prefix cache (``retire``).  Pages that other slots share stay theirs."""
+        s = self.slots[slot]
+        self.alloc.release(s.pages)
+        s.pages, s.tokens, s.filled = [], [], 0
+        s.active, s.retired_at = False, -1
+        self.cache_offsets[slot] = self.time_dim_sizes[slot] = 0
+        self.user_phase[slot] = PHASE_UNALLOCATED
+        self._write_row(slot)
+
+    def fork(self, slot: int) -> tuple[int, list[tuple[int, int]]]:
+        """A second sequence that continues where ``slot`` stands, in a free slot: several samples of
+        one prompt, or a beam.  Returns ``(new_slot, copies)``; the caller copies page ``src`` to
+        page ``dst`` for every ``(src, dst)`` of ``copies`` on the device
+        (``kernels.pages.copy_pages``), behind the steps launched so far and before the next.
+
+        Full pages are shared.  The page of the slot's last token is copied: the state may already
+        have been advanced to a token that only the next step writes (``advance_decode``), and both
+        sequences will write that row.  The new slot gets as many pages of its own behind it as the
+        old one has reserved."""
+        s = self.slots[slot]
+        if s.filled <= 0:
+            raise ValueError(f"slot {slot} holds no tokens")
+        free = [i for i in self.free_slots() if i != slot]
+        if not free:
+            raise RuntimeError("no free slot")
+        new = min(free, key=lambda i: len(self.slots[i].pages))
+        t = self.slots[new]
+        self.alloc.release(t.pages)
+        t.pages, t.tokens, t.filled, t.retired_at = [], [], 0, -1
+        self._write_row(new)
+        shared = (s.filled - 1) // self.page_size
+        need = len(s.pages) - shared
+        self._make_room(need, keep=slot)
+        own = self.alloc.alloc(need)
+        self.alloc.retain(s.pages[:shared])
+        t.pages = list(s.pages[:shared]) + own
+        t.tokens, t.filled, t.active = list(s.tokens), s.filled, True
+        self.cache_offsets[new], self.time_dim_sizes[new] = self.cache_offsets[slot], self.time_dim_sizes[slot]
+        self.user_phase[new] = self.user_phase[slot]
+        self._write_row(new)
+        return new, [(s.pages[shared], own[0])]
+
+    def compact(self) -> tuple[np.ndarray, np.ndarray]:
+        """Moves every page in use to the front of the pool, so that the pages behind
+        ``num_pages - free_pages`` hold nothing (a pool can then be shrunk, or its tail lent out).
+        Returns ``(src, dst)`` int32 page ids for ``kernels.pages.copy_pages``, to run behind the steps
+        launched so far and before the next, whose block tables are the new ones (``upload``).  No
+        page is both read and written."""
+        live = np.flatnonzero(self.alloc._refs > 0)
+        src = live[live >= len(live)].astype(np.int32)
+        holes = np.flatnonzero(self.alloc._refs[: len(live)] == 0)
+        dst = holes.astype(np.int32)
+        if len(src) == 0:
+            return src, dst
+        moved = np.arange(self.alloc.num_pages)
+        moved[src] = dst
+        for i, s in enumerate(self.slots):
+            if s.pages:
+                s.pages = [int(p) for p in moved[s.pages]]
+                self._write_row(i)
+        self.alloc.move(src, dst)
+        return src, dst
 
     def ensure(self, slot: int, n_tokens: int) -> bool:
         """Makes the slot's table cover ``n_tokens`` tokens.  Returns True if pages were added."""
@@ -223,6 +297,22 @@ class PagedKVManager:
                 s.filled = max(s.filled, int(time_sizes_after[b]))
         return self.block_tables, self.cache_offsets, self.time_dim_sizes, self.user_phase
 
+    def prepare_packed_inputs(self, row_counts, time_sizes_after):
+        """One packed step (``rope.rope_norm_append_packed``, ``fa2.flash_attention_packed``): slot b
+        brings ``row_counts[b]`` new rows, none if 0 (prompts, chunks and single tokens may mix), and
+        holds ``time_sizes_after[b]`` tokens after it.  Pages are added as ``prepare_prefill_inputs`` adds
+        them.  Returns ``(q_starts, block_tables, time_dim_sizes)``; ``q_starts [B+1]``."""
+        if len(row_counts) != self.max_batch or len(time_sizes_after) != self.max_batch:
+            raise ValueError("row_counts and time_sizes_after need an entry for every slot")
+        rows = [int(n) for n in row_counts]
+        after = [int(t) if n else 0 for n, t in zip(rows, time_sizes_after)]
+        for b, (n, t) in enumerate(zip(rows, after)):
+            if n < 0 or n > t and n:
+                raise ValueError(f"slot {b}: {n} new rows of {t} tokens")
+        self._prepare([t - n for n, t in zip(rows, after)], after, PHASE_PREFILL, reserve=0)
+        self.q_starts[1:] = np.cumsum(rows)
+        return self.q_starts, self.block_tables, self.time_dim_sizes
+
     def decode_steps_covered(self, slot: int) -> int:
         """How many more tokens the slot can append on the device before it needs a new page."""
         return len(self.slots[slot].pages) * self.page_size - int(self.time_dim_sizes[slot])
@@ -258,6 +348,7 @@ class PagedKVManager:
             "cache_offsets": torch.from_numpy(self.cache_offsets),
             "time_dim_sizes": torch.from_numpy(self.time_dim_sizes),
             "user_phase": torch.from_numpy(self.user_phase),
+            "q_starts": torch.from_numpy(self.q_starts),
         }
         self._staging = {k: (torch.empty_like(v).pin_memory() if pin else torch.empty_like(v)) for k, v in self._host.items()}
         self.device_tensors = {k: torch.empty_like(v, device=self._device) for k, v in self._host.items()}
@@ -272,7 +363,7 @@ class PagedKVManager:
         if self._copy_pending:
             self._copied.synchronize()      # the staging buffers are still being read
             self._copy_pending = False
-        for name in ("cache_offsets", "time_dim_sizes", "user_phase", "block_tables"):
+        for name in ("cache_offsets", "time_dim_sizes", "user_phase", "q_starts", "block_tables"):
             if name == "block_tables" and tables_only_if_dirty and not self.tables_dirty:
                 continue
             self._staging[name].copy_(self._host[name])

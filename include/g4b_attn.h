@@ -380,6 +380,72 @@ int g4b_attn_combine_exchange(const G4bExchangeArgs* args, void* cuda_stream);
 /* Bytes of one rank's exchange buffer for `rows` = B * H * Tq rows of `head_dim` elements. */
 int64_t g4b_exchange_buffer_bytes(int world, int64_t rows, int head_dim);
 
+/*
+ * Packed rows: prompts, chunks and single tokens of several slots behind one another, without
+ * padding.  Slot b brings rows [q_starts[b], q_starts[b+1]) of N (none if the two are equal); they
+ * are the last of its time_dim_sizes[b] tokens, so row i of slot b lies at place
+ * time_dim_sizes[b] - (q_starts[b+1] - i) of its paged cache.  q_starts int32 [B+1] must not
+ * decrease and must end at or before N; rows that no slot owns are neither read nor written.  No
+ * counterpart in the reference, which pads every slot's chunk to one length.
+ *
+ * g4b_rope_norm_append_packed: what g4b_rope_norm_append does, for packed rows and with rotary
+ * positions over several axes: pair (i, i + D/2) of row n turns by
+ *     positions[pair_axis[i]][n] * rope_freqs[i]
+ * (time, height and width for the patches of an image or a video).  The angle is reduced in 64
+ * bits, the sine and cosine are taken in 32.  Without positions a row's position is its place in
+ * the cache.  q goes to q_out, or back into q; k and v go to the pools.  A row whose place is
+ * outside the block table or whose table entry is outside the pool is not appended (0x101 / 0x102
+ * in the device status word); a pair_axis entry past the axes is taken as 0 (0x106).
+ */
+typedef struct G4bRopePackedArgs {
+  G4bTensor q;              /* [N, H, D] view, last stride 1; f32, f16 or bf16 */
+  G4bTensor k, v;           /* [N, G, D] views, q's type */
+  G4bTensor q_out;          /* optional [N, H, D] view, any float type */
+  G4bTensor rope_freqs;     /* f32 [D/2] */
+  G4bTensor positions;      /* optional int32 or int64 [axes, N] view */
+  G4bTensor pair_axis;      /* uint8 [D/2]; optional with one axis */
+  G4bTensor q_starts;       /* int32 [B+1] */
+  G4bTensor time_dim_sizes; /* int32 [B] */
+  G4bTensor q_norm_w;       /* optional f32 [D] */
+  G4bTensor k_norm_w;       /* optional f32 [D] */
+  G4bTensor k_pool, v_pool; /* [num_pages, G, page_size, D], one float type, contiguous */
+  G4bTensor block_tables;   /* int32 [B, max_pages] */
+  float rmsnorm_eps;
+  int32_t page_size;
+  int32_t norm_qk;
+  int32_t norm_v;
+} G4bRopePackedArgs;
+int g4b_rope_norm_append_packed(const G4bRopePackedArgs* args, void* cuda_stream);
+
+/*
+ * Pages copied on the device, in every pool of every layer in one launch:
+ *     pool[dst_pages[i]] = pool[src_pages[i]]      for every pool and every i
+ * A pool is num_pages runs of page_bytes bytes (a K or V pool [num_pages, G, page_size, D] of any
+ * type, or the scales [num_pages, G] of an 8-bit one), all pools with the same num_pages.  What
+ * forking a sequence and compacting a pool ask for (g4b_b200/paging.py); no counterpart in the
+ * reference, whose slots are ring buffers.
+ *
+ * An entry whose src or dst is negative is padding (a captured launch keeps its list length); one
+ * with src == dst is nothing to do.  An entry past the pool is skipped and recorded (0x104 in the
+ * device status word).  A page may be the source of many entries.  Where it is the destination
+ * of several the entry with the lowest index is carried out, and an entry whose source
+ * is another's destination is skipped; both are recorded (0x105).  Entries are looked at as the
+ * list gives them: a skipped one still makes its destination one that others may not read.
+ */
+typedef struct G4bPagePool {
+  void* ptr;
+  int64_t page_bytes;
+} G4bPagePool;
+typedef struct G4bPageCopyArgs {
+  const G4bPagePool* pools; /* host array of num_pools, read before the call returns */
+  int64_t num_pages;
+  G4bTensor src_pages;      /* int32 [n], n <= 2^20 */
+  G4bTensor dst_pages;      /* int32 [n] */
+  int32_t num_pools;
+  int32_t reserved;
+} G4bPageCopyArgs;
+int g4b_page_copy(const G4bPageCopyArgs* args, void* cuda_stream);
+
 /* Message of the last failing call on this thread ("" if none). No reference counterpart:
  * the reference raises Python exceptions from its wrappers (fa2.py:656-657). */
 const char* g4b_last_error_string(void);
