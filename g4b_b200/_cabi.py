@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
+import sys
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "lib" / "libg4b_attn.so"
@@ -192,12 +194,24 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_dtype_codes: dict = {}     # dtype objects seen so far: spelling one out costs more than the rest of a view
+
+
 def dtype_code(dt) -> int:
+    try:
+        code = _dtype_codes.get(dt)
+    except TypeError:            # a dtype that cannot be a key
+        code = None
+    if code is not None:
+        return code
     name = getattr(dt, "name", None) or str(dt)
     name = name.replace("torch.", "").replace("numpy.", "").lower()
     if name not in _DTYPE_NAMES:
         raise TypeError(f"unsupported dtype {dt!r}")
-    return _DTYPE_NAMES[name]
+    code = _DTYPE_NAMES[name]
+    if type(dt).__module__ == "torch":
+        _dtype_codes[dt] = code
+    return code
 
 
 def _strides(t) -> list[int]:
@@ -247,27 +261,49 @@ def _check_device(t) -> None:
                          "make its device current (torch.cuda.device) before the call")
 
 
+# a G4bTensor as bytes: pointer, 5 extents, 5 strides, rank, dtype.  Packed in one go: field by
+# field a view costs three times as much, and a call packs a dozen.
+_VIEW = struct.Struct("@P5q5qii")
+_PAD = [(0,) * i for i in range(6)]
+_ABSENT = bytes(_VIEW.size)
+assert _VIEW.size == ctypes.sizeof(G4bTensor)
+
+
+def views(*tensors) -> bytes:
+    """The C views of tensor-likes (None: not given) behind one another, as bytes."""
+    torch = sys.modules.get("torch")
+    current = None          # the current device, asked for once
+    out = []
+    for t in tensors:
+        if t is None:
+            out.append(_ABSENT)
+            continue
+        if torch is not None and isinstance(t, torch.Tensor):
+            if _validate_only_depth == 0:
+                device = t.get_device()
+                if current is None and device >= 0:
+                    current = torch.cuda.current_device()
+                if device < 0 or device != current:
+                    _check_device(t)
+            shape, strides = t.shape, t.stride()
+            n = len(shape)
+        else:
+            if not (hasattr(t, "shape") and hasattr(t, "stride") and hasattr(t, "dtype") and hasattr(t, "data_ptr")):
+                raise TypeError(f"expected a tensor-like with shape/stride/dtype/data_ptr, got {type(t).__name__}")
+            _check_device(t)
+            shape, strides = [int(x) for x in t.shape], [int(x) for x in _strides(t)]
+            n = len(shape)
+            strides = strides[:n] + [0] * (n - len(strides))
+        if n > 5:
+            raise ValueError("tensors of rank > 5 are not supported")
+        pad = _PAD[5 - n]
+        out.append(_VIEW.pack(int(t.data_ptr()), *shape, *pad, *strides, *pad, n, dtype_code(t.dtype)))
+    return b"".join(out)
+
+
 def as_tensor(t) -> G4bTensor:
     """Packs a tensor-like (or None) into the C view; strides are in elements."""
-    out = G4bTensor()
-    if t is None:
-        out.ptr = None
-        out.ndim = 0
-        return out
-    if not (hasattr(t, "shape") and hasattr(t, "stride") and hasattr(t, "dtype") and hasattr(t, "data_ptr")):
-        raise TypeError(f"expected a tensor-like with shape/stride/dtype/data_ptr, got {type(t).__name__}")
-    _check_device(t)
-    shape = list(t.shape)
-    if len(shape) > 5:
-        raise ValueError("tensors of rank > 5 are not supported")
-    strides = _strides(t)
-    out.ptr = int(t.data_ptr())
-    for i, (n, s) in enumerate(zip(shape, strides)):
-        out.shape[i] = int(n)
-        out.stride[i] = int(s)
-    out.ndim = len(shape)
-    out.dtype = dtype_code(t.dtype)
-    return out
+    return G4bTensor.from_buffer_copy(views(t))
 
 
 def current_stream(stream=None) -> int:

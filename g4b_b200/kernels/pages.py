@@ -4,18 +4,9 @@ reference, whose slots are ring buffers; the page lists come from ``g4b_b200.pag
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from g4b_b200 import _cabi
-
-
-def _pool(p, num_pages: int) -> tuple[int, int]:
-    """Address and bytes of a page of one pool.  Only torch tensors come here (the pools of every layer, dozens in a call),
-    so what is asked of a tensor is what costs least."""
-    if not p.is_contiguous():
-        raise ValueError("page pools must be contiguous")
-    if p.dim() < 1 or p.shape[0] != num_pages:
-        raise ValueError("page pools must all have the same number of pages (dim 0)")
-    return p.data_ptr(), (p.nbytes // num_pages if num_pages else 0)
 
 
 def copy_pages(pools, src_pages, dst_pages, *, stream=None):
@@ -27,18 +18,26 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status
     word says so), so what it does never depends on the order of the blocks.  Returns None."""
+    # (the pools are dozens: of each is asked what costs least)
     pools = list(pools)
-    num_pages = int(pools[0].shape[0]) if pools and len(pools[0].shape) else 0
-    a = _cabi.G4bPageCopyArgs()
+    num_pages = int(pools[0].shape[0]) if pools and pools[0].dim() else 0
+    flat = []
+    device = None
+    for p in pools:
+        if p.get_device() != device:
+            _cabi._check_device(p)
+            device = p.get_device()
+        if not p.is_contiguous():
+            raise ValueError("page pools must be contiguous")
+        shape = p.shape
+        if not shape or shape[0] != num_pages:
+            raise ValueError("page pools must all have the same number of pages (dim 0)")
+        flat += (p.data_ptr(), p.nbytes)
+    flat[1::2] = [n // max(num_pages, 1) for n in flat[1::2]]
+    table = (_cabi.G4bPagePool * len(pools)).from_buffer_copy(struct.pack(f"@{len(flat)}q", *flat))
+    a = _cabi.G4bPageCopyArgs(table, num_pages)
     a.src_pages = _cabi.as_tensor(src_pages)
     a.dst_pages = _cabi.as_tensor(dst_pages)
-    table = (_cabi.G4bPagePool * len(pools))()
-    for p in pools:
-        _cabi._check_device(p)
-    flat = [x for p in pools for x in _pool(p, num_pages)]
-    ctypes.memmove(table, (ctypes.c_int64 * len(flat))(*flat), 8 * len(flat))
-    a.pools = table
-    a.num_pages = num_pages
     a.num_pools = len(pools)
     _cabi.check(_cabi.load().g4b_page_copy(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
     return None

@@ -3,8 +3,11 @@ form that also normalises V and appends K and V to the cache in the same launch.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from g4b_b200 import _cabi
+
+_PACKED_TAIL = struct.Struct("@fiii")     # the end of G4bRopePackedArgs: eps, page_size, norm_qk, norm_v
 
 
 def _launch(a, stream):
@@ -132,28 +135,13 @@ def rope_norm_append_packed(
     ``pair_axis [D/2]`` (uint8) deals the pairs to time, height and width in sections or in turn.
     The rotated q goes to ``q_out`` (any float dtype) or back into ``q``; k and v go to their slots'
     pages.  No counterpart in the reference."""
-    a = _cabi.G4bRopePackedArgs()
-    a.q = _cabi.as_tensor(q)
-    a.k = _cabi.as_tensor(k)
-    a.v = _cabi.as_tensor(v)
-    a.q_out = _cabi.as_tensor(q_out)
-    a.rope_freqs = _cabi.as_tensor(rope_freqs)
-    a.positions = _cabi.as_tensor(positions)
-    if positions is not None and a.positions.ndim == 1:
-        a.positions.ndim = 2
-        a.positions.shape[1], a.positions.stride[1] = a.positions.shape[0], a.positions.stride[0]
-        a.positions.shape[0], a.positions.stride[0] = 1, 0
-    a.pair_axis = _cabi.as_tensor(pair_axis)
-    a.q_starts = _cabi.as_tensor(q_starts)
-    a.time_dim_sizes = _cabi.as_tensor(time_dim_sizes)
-    a.q_norm_w = _cabi.as_tensor(q_rmsnorm_w)
-    a.k_norm_w = _cabi.as_tensor(k_rmsnorm_w)
-    a.k_pool = _cabi.as_tensor(k_pool)
-    a.v_pool = _cabi.as_tensor(v_pool)
-    a.block_tables = _cabi.as_tensor(block_tables)
-    a.rmsnorm_eps = float(rmsnorm_eps)
-    a.page_size = int(page_size)
-    a.norm_qk = 1 if norm_qk else 0
-    a.norm_v = 1 if norm_v else 0
+    a = _cabi.G4bRopePackedArgs.from_buffer_copy(
+        _cabi.views(q, k, v, q_out, rope_freqs, positions, pair_axis, q_starts, time_dim_sizes, q_rmsnorm_w, k_rmsnorm_w,
+                    k_pool, v_pool, block_tables)
+        + _PACKED_TAIL.pack(rmsnorm_eps, page_size, 1 if norm_qk else 0, 1 if norm_v else 0))
+    if a.positions.ndim == 1:            # one axis
+        n, step = a.positions.shape[0], a.positions.stride[0]
+        a.positions.ndim, a.positions.shape[0], a.positions.stride[0] = 2, 1, 0
+        a.positions.shape[1], a.positions.stride[1] = n, step
     _cabi.check(_cabi.load().g4b_rope_norm_append_packed(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
     return None
