@@ -131,6 +131,14 @@ class G4bRopePackedArgs(ctypes.Structure):
     ]
 
 
+class G4bPackedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", G4bTensor), ("o", G4bTensor), ("k_pool", G4bTensor), ("v_pool", G4bTensor), ("q_starts", G4bTensor),
+        ("time_dim_sizes", G4bTensor), ("block_tables", G4bTensor), ("workspace", G4bTensor),
+        ("page_size", ctypes.c_int32), ("stage", ctypes.c_int32), ("sliding_window", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
 class G4bPagePool(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p), ("page_bytes", ctypes.c_int64)]
 
@@ -161,6 +169,8 @@ EXPORTS = {
     "g4b_rope_norm_append": (ctypes.c_int, [ctypes.POINTER(G4bRopeAppendArgs), ctypes.c_void_p]),
     "g4b_advance_decode_state": (ctypes.c_int, [ctypes.POINTER(G4bAdvanceArgs), ctypes.c_void_p]),
     "g4b_rope_norm_append_packed": (ctypes.c_int, [ctypes.POINTER(G4bRopePackedArgs), ctypes.c_void_p]),
+    "g4b_flash_attention_packed": (ctypes.c_int, [ctypes.POINTER(G4bPackedAttnArgs), ctypes.c_void_p]),
+    "g4b_packed_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
     "g4b_page_copy": (ctypes.c_int, [ctypes.POINTER(G4bPageCopyArgs), ctypes.c_void_p]),
     "g4b_last_error_string": (ctypes.c_char_p, []),
     "g4b_abi_version": (ctypes.c_int, []),

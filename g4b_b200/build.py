@@ -20,7 +20,7 @@ LIB = LIBDIR / "libg4b_attn.so"
 INCLUDE = PKG.parent / "include"
 
 SOURCES = ["api.cu", "kv_append.cu", "rope_append.cu", "combine.cu", "combine_exchange.cu", "decode.cu", "decode_stream.cu", "decode_static.cu", "tensor_map.cu", "prefill_sm100.cu",
-           "page_copy.cu", "rope_packed.cu"]
+           "page_copy.cu", "rope_packed.cu", "prefill_packed_sm100.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -74,6 +74,7 @@ int launch_kv_append_fp8(const G4bFp8AppendArgs& a, cudaStream_t st);
 int launch_kv_dequant_fp8(const G4bFp8DequantArgs& a, cudaStream_t st);
 int launch_prefill(const G4bAttnArgs& a, cudaStream_t st);
 int launch_rope_norm_append_packed(const G4bRopePackedArgs& a, cudaStream_t st);
+int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st);
 int launch_page_copy(const G4bPageCopyArgs& a, cudaStream_t st);
 
 // ---------------------------------------------------------------------------------------

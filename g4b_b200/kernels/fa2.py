@@ -10,6 +10,7 @@ count.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from g4b_b200 import _cabi
 
@@ -21,6 +22,8 @@ STAGE_CAUSAL = STAGE_FULL | STAGE_ON_BAND
 PHASE_UNALLOCATED = 0
 PHASE_PREFILL = 1
 PHASE_DECODE = 2
+
+_PACKED_TAIL = struct.Struct("@iiif")     # the end of G4bPackedAttnArgs: page_size, stage, sliding_window, scale
 
 
 def select_kv_splits(ctx_window_size: int, max_kv_splits: int, phase: int, tq: int) -> int:
@@ -191,3 +194,28 @@ def decode_attention_static_scratch(q, k_cache, v_cache, o, time_dim_sizes, user
                    None, None, None, stage, scale, sliding_window, block_tables, page_size, num_kv_splits)
     _cabi.check(_cabi.load().g4b_attn_decode_static_scratch(ctypes.byref(a),
                                                             ctypes.c_void_p(_cabi.current_stream(stream))))
+
+
+def packed_workspace_bytes(rows: int, slots: int, q_heads: int, kv_heads: int) -> int:
+    """Bytes of workspace that ``flash_attention_packed`` needs for up to ``rows`` packed rows of ``slots`` slots."""
+    n = int(_cabi.load().g4b_packed_workspace_bytes(int(rows), int(slots), int(q_heads), int(kv_heads)))
+    if n <= 0:
+        raise ValueError("rows and slots must not be negative, query heads a multiple (at most 128) of the kv heads")
+    return n
+
+
+def flash_attention_packed(q, k_pool, v_pool, o, q_starts, time_dim_sizes, *, block_tables, workspace, page_size: int = 16,
+                           scale: float = 1.0, sliding_window: int | None = None, stage: int = STAGE_CAUSAL, stream=None):
+    """Attention of packed rows ``q [N,H,D]`` into ``o`` over a paged cache (``g4b_flash_attention_packed``):
+    slot b owns rows ``[q_starts[b], q_starts[b+1])``, the last of its ``time_dim_sizes[b]`` tokens, whose K
+    and V rows are already in its pages.  Prompts, chunks behind a cached context and single tokens of
+    different slots mix freely; rows that no slot owns stay as they are.  No counterpart in the reference,
+    which pads every slot's chunk to one length.
+
+    ``workspace``: device memory of at least ``packed_workspace_bytes(N, B, H, G)`` bytes, which a program
+    allocates once; calls that may overlap on the GPU need one each.  Returns None."""
+    a = _cabi.G4bPackedAttnArgs.from_buffer_copy(
+        _cabi.views(q, o, k_pool, v_pool, q_starts, time_dim_sizes, block_tables, workspace)
+        + _PACKED_TAIL.pack(page_size, stage, sliding_window or 0, scale))
+    _cabi.check(_cabi.load().g4b_flash_attention_packed(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
+    return None

@@ -418,6 +418,38 @@ typedef struct G4bRopePackedArgs {
 int g4b_rope_norm_append_packed(const G4bRopePackedArgs* args, void* cuda_stream);
 
 /*
+ * g4b_flash_attention_packed: attention of packed rows (see above) over the slots' pages, whose K and V
+ * rows are in place (g4b_rope_norm_append_packed, or g4b_kv_append): row i of slot b, at position
+ * p = time_dim_sizes[b] - (q_starts[b+1] - i), attends to keys j < time_dim_sizes[b], j <= p
+ * (stage causal), j > p - sliding_window (if not 0).  A row that sees no key is zero.  tcgen05 / TMEM /
+ * TMA, head dims 128 and 256, f16 or bf16 pools, q of their type, o of their type or f32, up to 128 query
+ * heads per kv head.  The padded form with a ring, f32 q and other features is g4b_flash_attention.
+ *
+ * workspace: at least g4b_packed_workspace_bytes(N, B, H, G) bytes of any type, 16-byte aligned; it
+ * needs no initial contents and keeps none between calls, but calls that overlap on the GPU (two streams,
+ * two captured graphs replayed side by side) each need their own.
+ *
+ * q_starts that decrease or leave [0, N]: nothing is computed, 0x107 in the device status word.  A
+ * block-table entry outside the pool reads as zeros and is recorded (0x309), a slot is attended to as
+ * far as its table reaches.
+ */
+typedef struct G4bPackedAttnArgs {
+  G4bTensor q, o;           /* [N, H, D] views, last stride 1, other strides positive multiples of 16 bytes */
+  G4bTensor k_pool, v_pool; /* [num_pages, G, page_size, D] contiguous */
+  G4bTensor q_starts;       /* int32 [B+1] */
+  G4bTensor time_dim_sizes; /* int32 [B] */
+  G4bTensor block_tables;   /* int32 [B, max_pages] */
+  G4bTensor workspace;
+  int32_t page_size;
+  int32_t stage;
+  int32_t sliding_window;
+  float scale;
+} G4bPackedAttnArgs;
+int g4b_flash_attention_packed(const G4bPackedAttnArgs* args, void* cuda_stream);
+/* 0 when the head counts are not ones the call takes */
+int64_t g4b_packed_workspace_bytes(int64_t rows, int64_t slots, int q_heads, int kv_heads);
+
+/*
  * Pages copied on the device, in every pool of every layer in one launch:
  *     pool[dst_pages[i]] = pool[src_pages[i]]      for every pool and every i
  * A pool is num_pages runs of page_bytes bytes (a K or V pool [num_pages, G, page_size, D] of any
