@@ -35,7 +35,7 @@ namespace {
 
 constexpr int kBM = 128;           // rows per CTA: (token, head) pairs
 constexpr int kBN = 128;           // keys per S tile
-constexpr int kThreads = 320;      // producer warp, MMA warp, 2 softmax warpgroups
+constexpr int kThreads = 352;      // producer warps 0 (Q and K) and 10 (V), MMA warp 1, 2 softmax warpgroups
 constexpr int kStageBytes = 8 * 4096;         // output: 4 KB per softmax warp
 constexpr int kXchgBytes = 2 * 2 * kBM * 4;   // row maxima: [tile parity][column half][row]
 
@@ -327,8 +327,12 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     if (lane == 0) ptx::mbar_arrive_cluster_relaxed(bar);
   };
 
-  if (warp == 0) {
-    // =============================== producer ===============================
+  if (warp == 0 || warp == 10) {
+    // =============================== producers ===============================
+    // Warp 0 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB, 32 of them a tile, and one
+    // warp does not issue them as fast as the tensor pipe consumes them (4 prompts of 8192 rows, 8 / 2 heads,
+    // pages of 16: 1153 us with one producer warp, 846 us with two).
+    const bool for_k = warp == 0, for_v = warp == 10;
     const uint64_t pol_kv = ptx::policy_evict_last();    // K/V tiles are re-read by every block of the slot
     const uint64_t pol_q = ptx::policy_evict_first();
     const uint32_t q_bytes = (uint32_t)(kSlabs * p.tpt * p.group * 128);
@@ -352,8 +356,8 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         return w != 0;
       };
       // the Q buffer is free once the last Q.K^T of the previous item has run
-      if (n_done > 0 && !wait_lane0(ptx::smem_u32(&bars->q_empty), (n_done - 1) & 1, kErrQEmpty)) break;
-      if (lane == 0) {
+      if (for_k && n_done > 0 && !wait_lane0(ptx::smem_u32(&bars->q_empty), (n_done - 1) & 1, kErrQEmpty)) break;
+      if (for_k && lane == 0) {
         const uint32_t qb = issuer_bar(&bars->q_full);
         ptx::mbar_arrive_expect_tx_cluster(qb, q_bytes);
         for (int s = 0; s < kSlabs; ++s)
@@ -373,6 +377,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       // this CTA's half of the head dim (slabs of [128 rows x 64 d]).  Lane i fetches the i-th group of
       // rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
       auto load_k = [&](int j) {
+        if (!for_k) { ++cc; return; }
         const int key0 = (it.tile_lo + j) * kBN + 64 * (int)rank + lane * p.k_rows;
         const int boxes = 64 / p.k_rows;
         const int page = lane < boxes ? page_of(key0) : 0;
@@ -391,6 +396,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         ++cc;
       };
       auto load_v = [&](int j) {
+        if (!for_v) { ++cc; return; }
         const int tile0 = (it.tile_lo + j) * kBN;
         const int key0 = tile0 + lane * p.v_rows;
         const int boxes = kBN / p.v_rows;
@@ -596,13 +602,17 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     // any reference in that range is as good as the maximum itself -- so the first tile of an item
     // can take the optimistic path too.
     float m_carry = -INFINITY;
+    // (the next entry is fetched behind the tile loop, where registers are free, and arrives during the epilogue)
     G4B_PACKED_LOOP_PROLOGUE();
     for (int round = 0; round * n_workers < n_items && ok; ++round) {
-      G4B_PACKED_LOOP_HEAD(round);
+      const int item = item_of_round(round);
+      const PackedItem it = it_nx_;
+      auto fetch_next = [&]() { fetch_item((round + 1) * n_workers < n_items ? item_of_round(round + 1) : -1, it_nx_); };
       if (item < 0) continue;
       const int g = item % p.G;
       const int n_tiles = it.n_tiles;
       if (n_tiles <= 0) {
+        fetch_next();
         // no visible key for any row of the block: the output rows are zero
         *reinterpret_cast<uint4*>(stage + lane * 128) = make_uint4(0u, 0u, 0u, 0u);
         for (int c = 1; c < 8; ++c) *reinterpret_cast<uint4*>(stage + lane * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -793,6 +803,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       }
 
       if (!few_keys && m_used != -INFINITY) m_carry = m_used;
+      fetch_next();
       // ---- epilogue: O / l -> global ----
       if (ok) {
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (tg + n_tiles - 1) & 1))) { record(p.status, kErrPvDone); ok = false; }
@@ -826,24 +837,26 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
           ptx::tc_fence_before();
           arrive_issuer(issuer_bar(&bars->o_free));
         } else {
-          // O out of tensor memory first (normalised and packed): the next item's first P.V overwrites it
-          uint32_t pk[kHalfCols / 32][16];
-#pragma unroll
-          for (int c = 0; c < kHalfCols / 32; ++c) {
-            uint32_t ov[32];
-            ptx::tmem_ld32(o_col + c * 32, ov);
-            ptx::tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              pk[c][i] = PackT<T>::pack(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l);
-          }
-          ptx::tc_fence_before();
-          arrive_issuer(issuer_bar(&bars->o_free));
 #pragma unroll
           for (int c = 0; c < kHalfCols / 64; ++c) {
+            uint32_t pk[2][16];
+#pragma unroll
+            for (int c2 = 0; c2 < 2; ++c2) {
+              uint32_t ov[32];
+              ptx::tmem_ld32(o_col + (2 * c + c2) * 32, ov);
+              ptx::tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                pk[c2][i] = PackT<T>::pack(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l);
+            }
+            if (c == kHalfCols / 64 - 1) {
+              // O is out of tensor memory: the next item's first P.V may overwrite it
+              ptx::tc_fence_before();
+              arrive_issuer(issuer_bar(&bars->o_free));
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const uint32_t* x = &pk[2 * c + (i >> 2)][(i & 3) * 4];
+              const uint32_t* x = &pk[i >> 2][(i & 3) * 4];
               put(i, x[0], x[1], x[2], x[3]);
             }
             store_stage(it, g, (half * kHalfCols + c * 64) * 2);
