@@ -16,8 +16,11 @@
 //   box of the packed q.  All heads of a group share the tile, so one token is one row per head
 //   instead of a tile per head, and the ragged end of a causal block is 2 x 128 / (H/G) tokens wide.
 // Items.  A work item is a block of tokens of one slot and one kv head.  How many there are is known
-//   on the device only; a small launch before this one (plan_kernel) lists them, those with most keys
-//   first, so that the static walk over the list stays balanced whatever the mix of lengths.
+//   on the device only; a small launch before this one (plan_kernel) lists them.  With enough of them they
+//   are dealt whole, those with most keys first.  Where a few long ones would keep some workers busy
+//   long after the others (chunks behind long contexts, single tokens), every worker gets the same share of
+//   the tiles instead: an item that lies across a boundary leaves its un-normalised parts in the
+//   workspace, and a third launch joins them.
 // Pages.  A box is one page's rows (up to what a CTA stages); groups of rows past the context, and
 //   groups whose table entry is bad, are boxes outside the pool, which TMA fills with zeros.  Where the
 //   context ends inside a group the producer zeroes the rest of V itself (it may hold anything, and
@@ -55,26 +58,52 @@ enum : int32_t {
   kErrSmemAlign = 0x307, kErrPair = 0x308, kErrBadPage = 0x309, kErrQEmpty = 0x30a, kErrOFree = 0x30b, kErrTail = 0x30d,
 };
 
-// One block of tokens of one slot, for every kv head.
+// One block of tokens of one slot and kv head, or a piece of its keys.
 struct __align__(16) PackedItem {
-  int row0, n_tok;        // its rows of q and o
+  int row0, n_tok;        // its rows of q and o (n_tok 0: an entry without work)
   int qpos0;              // position of the first
   int window;             // keys [0, window) exist
   int tile_lo, n_tiles;   // its 128-key tiles
-  int slot, pad;
+  int slot;
+  int g_part;             // kv head; upper 16 bits: 0, or 1 + the part of the workspace that this piece leaves
 };
 
-// Workspace: a header of 16 words (word 0: number of items per kv head), then the items.
-constexpr int kHeaderBytes = 64;
+// The pieces of one split item.
+struct JoinEntry {
+  int row0, n_tok, g;
+  int w_lo, w_hi;         // workers that hold a piece
+  int part_lo;            // the first one's part; worker w > w_lo left part 2 w
+  int pad[2];
+};
+
+constexpr int kMaxWorkers = 74;          // CTA pairs of a 148-SM GPU
+constexpr int kMaxSplitItems = 2048;     // items (per kv head) up to which shares are dealt
+constexpr int kPartRows = 2 * kBM;
+
+// Workspace, in this order: counts, what each worker walks, split items, (l, m) of the parts, the parts,
+// the list (the only piece whose size depends on the call).
+struct PackedHeader {
+  int n_entries;          // whole items, dealt in turns (walks absent)
+  int shares;             // 1: worker w walks entries [begin[w], end[w])
+  int n_joins;
+  int pad[13];
+  int begin[kMaxWorkers], end[kMaxWorkers];
+  JoinEntry joins[kMaxWorkers];
+  float part_lm[2 * kMaxWorkers][kPartRows][2];
+};
+constexpr int64_t kPartsAt = (sizeof(PackedHeader) + 255) / 256 * 256;
+constexpr int64_t kPartBytes = (int64_t)kPartRows * 256 * 4;       // head dim 256; 128 uses half
+constexpr int64_t kItemsAt = kPartsAt + 2 * kMaxWorkers * kPartBytes;
 
 struct PackedParams {
   void* o;
   const int32_t* q_starts; const int32_t* times; const int32_t* block_tables;
-  int32_t* header; PackedItem* items;
+  PackedHeader* header; float* parts; PackedItem* items;
   int64_t o_row, o_head, starts_s, time_s, bt_s0, bt_s1;
   int N, B, H, G;
   int group, tpt;                 // query heads per kv head; tokens per CTA (kBM / group)
-  int max_items;
+  int max_items, workers;
+  int may_split;                  // few enough blocks that shares can pay; then a join launch follows
   int page_shift, num_pages, max_pages;
   int k_rows, v_rows;             // rows of a K / V box
   int sliding_window, causal, o_dtype;
@@ -106,23 +135,185 @@ __device__ __forceinline__ SlotRows slot_rows(const PackedParams& p, int b) {
   return s;
 }
 
-// Items sorted by the position they end at (heaviest first; under a sliding window everything past
-// the window weighs the same).  Within a slot that position grows by `block` from item to item, so how
-// many items of another slot come before a given one is a closed form, and one warp ranks an
-// item with one look at every slot: no sort, no pass in between, any number of warps at once.
+// Which 128-key tiles a block of tokens at positions [qpos0, qpos0 + n_tok) needs.
+__device__ __forceinline__ void tiles_of(const PackedParams& p, int qpos0, int n_tok, int window, int& lo, int& n) {
+  const int key_hi = p.causal ? min(window, qpos0 + n_tok) : window;
+  const int key_lo = p.sliding_window > 0 ? max(0, qpos0 - p.sliding_window + 1) : 0;
+  lo = key_lo / kBN;
+  n = key_hi > key_lo ? (key_hi + kBN - 1) / kBN - lo : 0;
+}
+
+__device__ __forceinline__ PackedItem block_of(const PackedParams& p, const SlotRows& s, int slot, int index, int block) {
+  PackedItem it;
+  const int tok0 = index * block;
+  it.row0 = s.first + tok0;
+  it.n_tok = min(block, s.n - tok0);
+  it.qpos0 = s.time - s.n + tok0;
+  it.window = s.time;
+  tiles_of(p, it.qpos0, it.n_tok, it.window, it.tile_lo, it.n_tiles);
+  it.slot = slot;
+  it.g_part = 0;
+  return it;
+}
+
+// Over the block's 256 threads: the sum of the values before this thread's (kMax: the maximum up to and with
+// this thread's), and of all.
+template <bool kMax, typename V>
+__device__ __forceinline__ V block_scan(V x, V* warp_sums, V& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  V sum = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum = kMax ? max(sum, y) : sum + y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  V before = kMax ? sum : 0;
+  total = kMax ? sum : 0;
+  for (int w = 0; w < 8; ++w) {
+    const V y = warp_sums[w];
+    if (w < warp) before = kMax ? max(before, y) : before + y;
+    total = kMax ? max(total, y) : total + y;
+  }
+  return kMax ? before : before + sum - x;
+}
+
+constexpr int kEntryCost = 2;      // an item's start and epilogue, in tiles
+
+// Every worker the same share of the cost (tiles + kEntryCost an item) along the line of all items, slot by
+// slot and head by head; one block.  The entry of unit u (item, kv head) for worker w is u + w: along
+// the line either the unit or the worker goes up by one.
+__device__ __noinline__ void deal_shares(const PackedParams& p, int n_items) {
+  __shared__ int slot_of[kMaxSplitItems], start_of[kMaxSplitItems];      // an item's slot, and the slot's first item
+  __shared__ long long cost_before[kMaxSplitItems + 1];
+  __shared__ long long sums[8];
+  __shared__ int sums32[8], n_joins;
+  const int tid = threadIdx.x, block = 2 * p.tpt;
+  for (int i = tid; i < n_items; i += 256) slot_of[i] = -1;
+  if (tid == 0) n_joins = 0;
+  int at = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 256) {                 // (the scan's barriers order the -1 before the marks)
+    const SlotRows s = slot_rows(p, b0 + tid);
+    const int n = (s.n + block - 1) / block;
+    int all_here;
+    const int before = block_scan<false>(n, sums32, all_here);
+    if (n > 0) slot_of[at + before] = b0 + tid;
+    at += all_here;
+  }
+  __syncthreads();
+  long long total = 0;
+  int last_start = 0;
+  for (int i0 = 0; i0 < n_items; i0 += 256) {
+    const int i = i0 + tid;
+    int start, unused;
+    {
+      const int marked = i < n_items && slot_of[i] >= 0 ? i : last_start;
+      start = block_scan<true>(marked, sums32, unused);
+    }
+    long long c = 0, here;
+    if (i < n_items) {
+      const int slot = slot_of[start];
+      start_of[i] = start;
+      c = block_of(p, slot_rows(p, slot), slot, i - start, block).n_tiles + kEntryCost;
+    }
+    const long long before = block_scan<false>(c, sums, here);
+    if (i < n_items) cost_before[i] = total + before;
+    total += here;
+    last_start = unused;
+  }
+  if (tid == 0) cost_before[n_items] = total;
+  __syncthreads();
+  const long long all = total * p.G;
+  const long long share = max((all + p.workers - 1) / p.workers, (long long)(4 + kEntryCost));
+  // unit that holds the point x of the line
+  auto unit_at = [&](long long x) -> int {
+    int lo = 0, n = n_items;
+    while (n > 1) {
+      const int h = n / 2;
+      if (cost_before[lo + h] * p.G <= x) { lo += h; n -= h; } else { n = h; }
+    }
+    const long long c = cost_before[lo + 1] - cost_before[lo];
+    return lo * p.G + (int)((x - cost_before[lo] * p.G) / c);
+  };
+  for (int w = tid; w < p.workers; w += 256) {
+    const long long a = w * share, e = min(a + share, all);
+    p.header->begin[w] = a < all ? unit_at(a) + w : 0;
+    p.header->end[w] = a < all ? unit_at(e - 1) + w + 1 : 0;
+  }
+  for (int u = tid; u < n_items * p.G; u += 256) {
+    const int item = u / p.G, g = u - item * p.G;
+    const long long c = cost_before[item + 1] - cost_before[item];
+    const long long from = cost_before[item] * p.G + g * c;
+    const int st = start_of[item], slot = slot_of[st];
+    const PackedItem it = block_of(p, slot_rows(p, slot), slot, item - st, block);
+    const int n = it.n_tiles, lo_all = it.tile_lo;
+    // tiles in front of the point `x` of the item; pieces of one tile are not worth their epilogue
+    auto tiles_before = [&](long long x) -> int {
+      const long long t = x - kEntryCost / 2;
+      return t < 2 ? 0 : t > n - 2 ? n : (int)t;
+    };
+    const int w1 = (int)(from / share), w2 = (int)((from + c - 1) / share);
+    auto cut = [&](int w) { return tiles_before(min(max((long long)w * share - from, 0ll), c)); };
+    int w_lo = -1, w_hi = -1;
+    for (int w = w1; w <= w2; ++w)
+      if (cut(w) < cut(w + 1)) { if (w_lo < 0) w_lo = w; w_hi = w; }
+    for (int w = w1; w <= w2; ++w) {
+      const int lo = cut(w), hi = cut(w + 1);
+      PackedItem piece = it;
+      int part = 0;
+      if (lo < hi) {
+        piece.tile_lo = lo_all + lo;
+        piece.n_tiles = hi - lo;
+        if (w_lo < w_hi) part = 1 + (w == w1 && from > w1 * share ? 2 * w + 1 : 2 * w);
+      } else if (n > 0 || w > w1) {
+        piece.n_tok = piece.n_tiles = 0;
+      }
+      piece.g_part = g | (part << 16);
+      p.items[u + w] = piece;
+    }
+    if (w_lo < w_hi) {
+      JoinEntry j;
+      j.row0 = it.row0; j.n_tok = it.n_tok; j.g = g;
+      j.w_lo = w_lo; j.w_hi = w_hi;
+      j.part_lo = w_lo == w1 && from > w1 * share ? 2 * w_lo + 1 : 2 * w_lo;
+      j.pad[0] = j.pad[1] = 0;
+      p.header->joins[atomicAdd(&n_joins, 1)] = j;       // (every split item lies on a boundary of its own: fewer than workers)
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.header->n_entries = 0;
+    p.header->shares = 1;
+    p.header->n_joins = n_joins;
+  }
+}
+
+// Lists the items.  Whole ones are sorted by the position they end at (heaviest first; under a sliding
+// window everything past the window weighs the same).  Within a slot that position grows by `block` from
+// item to item, so how many items of another slot come before a given one is a closed form, and one
+// warp ranks an item with one look at every slot: no sort, no pass in between, any number of warps.
 __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ PackedParams p) {
   let_next_launch_start();
   const int lane = threadIdx.x & 31;
   const int warp = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int block = 2 * p.tpt;
   const int cap = p.sliding_window > 0 ? min(p.sliding_window, 0x40000000) + 2 * kBN : 0x7fffffff;
-  // which slot and which of its items: a scan over the slots' item counts
-  int at = 0, mine = -1, slot = 0;
+  // which slot and which of its items: a scan over the slots' item counts.  On the way: the longest item and
+  // (nearly) the cost of all, both in tiles
+  int at = 0, mine = -1, slot = 0, longest = 0;
+  float cost = 0.f;
   bool bad = false;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const SlotRows s = slot_rows(p, b0 + lane);
     bad |= s.bad;
     const int n = (s.n + block - 1) / block;
+    if (n > 0) {
+      const int last = min(s.time, cap), first = p.causal ? min(max(s.time - s.n + block, 0), last) : last;
+      longest = max(longest, (last + kBN - 1) / kBN);
+      cost += (float)n * ((float)(first + last) / (2 * kBN) + 0.5f + kEntryCost);
+    }
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -138,14 +329,30 @@ __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ Packe
     at += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (__any_sync(0xffffffffu, bad)) {          // starts that contradict themselves: nothing is computed
-    if (warp == 0 && lane == 0) { record(p.status, kErrStarts); p.header[0] = 0; }
+    if (warp == 0 && lane == 0) {
+      record(p.status, kErrStarts);
+      p.header->n_entries = p.header->shares = p.header->n_joins = 0;
+    }
     return;
   }
-  if (warp == 0 && lane == 0) p.header[0] = at;   // (at <= N / block + B: the starts do not decrease)
+  if (p.may_split) {
+    // Shares pay where the longest item alone takes longer than its worker's fair part of everything (and is
+    // worth cutting at all): chunks of 1 to 512 rows behind contexts of 777 to 30000 tokens, 8 / 2 heads: 573 us
+    // whole.  Every warp comes to the same answer.
+    longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+    if (longest > 8 && at <= kMaxSplitItems && (float)(longest + kEntryCost) * p.workers > 1.1f * cost * p.G) {
+      if (blockIdx.x == 0) deal_shares(p, at);
+      return;
+    }
+  }
+  if (warp == 0 && lane == 0) {
+    p.header->n_entries = at * p.G;            // (at <= N / block + B: the starts do not decrease)
+    p.header->shares = p.header->n_joins = 0;
+  }
   if (mine < 0) return;
   const SlotRows s = slot_rows(p, slot);
-  const int tok0 = mine * block, n_tok = min(block, s.n - tok0);
-  const int base = s.time - s.n;                  // position of the slot's first row
   auto ends_at = [&](int time, int n, int i) { return p.causal ? time - n + min((i + 1) * block, n) : time; };
   const int x = min(ends_at(s.time, s.n, mine), cap);
   int rank = 0;
@@ -160,19 +367,12 @@ __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ Packe
     if (b == slot) rank += min(max(mine - below, 0), same);
   }
   rank = __reduce_add_sync(0xffffffffu, rank);
-  if (lane != 0) return;
-  PackedItem it;
-  it.row0 = s.first + tok0;
-  it.n_tok = n_tok;
-  it.qpos0 = base + tok0;
-  it.window = s.time;
-  const int key_hi = p.causal ? min(it.window, it.qpos0 + n_tok) : it.window;
-  const int key_lo = p.sliding_window > 0 ? max(0, it.qpos0 - p.sliding_window + 1) : 0;
-  it.tile_lo = key_lo / kBN;
-  it.n_tiles = key_hi > key_lo ? (key_hi + kBN - 1) / kBN - it.tile_lo : 0;
-  it.slot = slot;
-  it.pad = 0;
-  if (rank < p.max_items) p.items[rank] = it;
+  PackedItem it = block_of(p, s, slot, mine, block);
+  if (rank < p.max_items)
+    for (int g = lane; g < p.G; g += 32) {
+      it.g_part = g;
+      p.items[(int64_t)rank * p.G + g] = it;
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -222,8 +422,8 @@ template <> struct PackT<__half> {
   }
 };
 
-// A worker's walk over the items: round r hands item r * workers + w to worker w, alternating the
-// direction so that heavy and light ones pair up.  The entry is read one item ahead: fetched at
+// A worker's walk: its share of the line of items or, of whole items, item r * workers + w in round r,
+// alternating the direction so that heavy and light ones pair up.  The entry is read one item ahead: fetched at
 // the switch itself, the load would hold up the MMA issuer and the softmax warps.
 #define G4B_PACKED_LOOP_PROLOGUE()                                                                   \
   PackedItem it_nx_;                                                                                 \
@@ -231,7 +431,7 @@ template <> struct PackT<__half> {
 #define G4B_PACKED_LOOP_HEAD(round)                                                                  \
   const int item = item_of_round(round);                                                             \
   const PackedItem it = it_nx_;                                                                      \
-  fetch_item(((round) + 1) * n_workers < n_items ? item_of_round((round) + 1) : -1, it_nx_)
+  fetch_item(item_of_round((round) + 1), it_nx_)
 
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -302,17 +502,22 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
 
   wait_for_launch_before();             // the list of items is complete
-  const int n_items = *reinterpret_cast<volatile int32_t*>(p.header) * p.G;
+  let_next_launch_start();
   const int n_workers = (int)gridDim.x / 2, worker = (int)blockIdx.x / 2;
+  const bool shares = __ldcg(&p.header->shares) != 0;
+  const int first_entry = shares ? __ldcg(&p.header->begin[worker]) : 0;
+  const int last_entry = shares ? __ldcg(&p.header->end[worker]) : __ldcg(&p.header->n_entries);
+  const int n_rounds = shares ? last_entry - first_entry : (last_entry + n_workers - 1) / n_workers;
   auto item_of_round = [&](int round) -> int {
-    const int item = round * n_workers + ((round & 1) ? n_workers - 1 - worker : worker);
-    return item < n_items ? item : -1;
+    if (round >= n_rounds) return -1;
+    const int item = shares ? first_entry + round : round * n_workers + ((round & 1) ? n_workers - 1 - worker : worker);
+    return item < last_entry ? item : -1;
   };
   auto fetch_item = [&](int item, PackedItem& out) {
     if (item < 0) { out.n_tok = 0; out.n_tiles = 0; return; }
-    const int4* src = reinterpret_cast<const int4*>(p.items + item / p.G);
+    const int4* src = reinterpret_cast<const int4*>(p.items + item);
     const int4 a = __ldcg(src), c = __ldcg(src + 1);
-    out = PackedItem{a.x, a.y, a.z, a.w, c.x, c.y, c.z, 0};
+    out = PackedItem{a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
   };
   // rows of the block that see fewer than 64 keys: the precise path (for the whole block, both CTAs)
   auto sees_few = [&](const PackedItem& x) {
@@ -342,10 +547,10 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     int n_done = 0;
     bool ok = true;
     G4B_PACKED_LOOP_PROLOGUE();
-    for (int round = 0; round * n_workers < n_items && ok; ++round) {
+    for (int round = 0; round < n_rounds && ok; ++round) {
       G4B_PACKED_LOOP_HEAD(round);
       if (item < 0 || it.n_tiles <= 0) continue;
-      const int g = item % p.G;
+      const int g = it.g_part & 0xffff;
       const int32_t* bt = p.block_tables + it.slot * p.bt_s0;
       const int page_mask = (1 << p.page_shift) - 1;
       auto wait_lane0 = [&](uint32_t bar, uint32_t parity, int32_t code) -> bool {
@@ -470,7 +675,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       int tg = 0;       // tiles issued so far: S buffer and barrier phases run on across items
       int n_done = 0;
       G4B_PACKED_LOOP_PROLOGUE();
-      for (int round = 0; round * n_workers < n_items && ok; ++round) {
+      for (int round = 0; round < n_rounds && ok; ++round) {
         G4B_PACKED_LOOP_HEAD(round);
         if (item < 0 || it.n_tiles <= 0) continue;
         const int n_tiles = it.n_tiles;
@@ -580,7 +785,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     // Stores 32 rows x 128 bytes out of this warp's stage: eight lanes a row, so that a row piece is one
     // whole line.  `bytes0`: offset of the piece inside an output row.
     const int osz = p.o_dtype == G4B_F32 ? 4 : 2;
-    auto store_stage = [&](const PackedItem& it, int g, int bytes0) {
+    auto store_stage = [&](const PackedItem& it, int g, int part, int bytes0) {
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -588,7 +793,9 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const int rr = lane_base + row, tok = (int)rank * p.tpt + rr / p.group;
         if (rr < p.tpt * p.group && tok < it.n_tok) {
           const uint4 val = *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
-          char* dst = (char*)p.o + ((int64_t)(it.row0 + tok) * p.o_row + (int64_t)(g * p.group + rr % p.group) * p.o_head) * osz + bytes0 + c * 16;
+          char* dst = part > 0 ? (char*)p.parts + (int64_t)(part - 1) * kPartBytes + ((int)rank * kBM + rr) * (kD * 4)
+                               : (char*)p.o + ((int64_t)(it.row0 + tok) * p.o_row + (int64_t)(g * p.group + rr % p.group) * p.o_head) * osz;
+          dst += bytes0 + c * 16;
           *reinterpret_cast<uint4*>(dst) = val;
         }
       }
@@ -604,19 +811,19 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     float m_carry = -INFINITY;
     // (the next entry is fetched behind the tile loop, where registers are free, and arrives during the epilogue)
     G4B_PACKED_LOOP_PROLOGUE();
-    for (int round = 0; round * n_workers < n_items && ok; ++round) {
+    for (int round = 0; round < n_rounds && ok; ++round) {
       const int item = item_of_round(round);
       const PackedItem it = it_nx_;
-      auto fetch_next = [&]() { fetch_item((round + 1) * n_workers < n_items ? item_of_round(round + 1) : -1, it_nx_); };
+      auto fetch_next = [&]() { fetch_item(item_of_round(round + 1), it_nx_); };
       if (item < 0) continue;
-      const int g = item % p.G;
+      const int g = it.g_part & 0xffff;
       const int n_tiles = it.n_tiles;
       if (n_tiles <= 0) {
         fetch_next();
         // no visible key for any row of the block: the output rows are zero
         *reinterpret_cast<uint4*>(stage + lane * 128) = make_uint4(0u, 0u, 0u, 0u);
         for (int c = 1; c < 8; ++c) *reinterpret_cast<uint4*>(stage + lane * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-        for (int c = 0; c < kHalfCols * osz / 128; ++c) store_stage(it, g, half * kHalfCols * osz + c * 128);
+        for (int c = 0; c < kHalfCols * osz / 128; ++c) store_stage(it, g, 0, half * kHalfCols * osz + c * 128);
         continue;
       }
       const int window = it.window;
@@ -822,17 +1029,23 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         auto put = [&](int c, uint32_t a, uint32_t b2, uint32_t c2, uint32_t d) {
           *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(a, b2, c2, d);
         };
-        if (p.o_dtype == G4B_F32) {
+        const int part = it.g_part >> 16;
+        if (part > 0 || p.o_dtype == G4B_F32) {
+          // f32 rows: an output of that type, or a part (un-normalised, with its sum and reference maximum in
+          // log2 units; a row that saw no key here has neither)
+          const float factor = part > 0 ? 1.f : inv_l;
+          if (part > 0 && half == 0 && in_tile && tok_r < it.n_tok)
+            *reinterpret_cast<float2*>(p.header->part_lm[part - 1][(int)rank * kBM + r]) = make_float2(l_run, l_run == 0.f ? -INFINITY : m_used);
 #pragma unroll 1
           for (int c = 0; c < kHalfCols / 32; ++c) {
             uint32_t ov[32];
             ptx::tmem_ld32(o_col + c * 32, ov);
             ptx::tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * inv_l);
+            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * factor);
 #pragma unroll
             for (int i = 0; i < 8; ++i) put(i, ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
-            store_stage(it, g, (half * kHalfCols + c * 32) * 4);
+            store_stage(it, g, part, (half * kHalfCols + c * 32) * 4);
           }
           ptx::tc_fence_before();
           arrive_issuer(issuer_bar(&bars->o_free));
@@ -859,7 +1072,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
               const uint32_t* x = &pk[i >> 2][(i & 3) * 4];
               put(i, x[0], x[1], x[2], x[3]);
             }
-            store_stage(it, g, (half * kHalfCols + c * 64) * 2);
+            store_stage(it, g, 0, (half * kHalfCols + c * 64) * 2);
           }
         }
       }
@@ -876,6 +1089,44 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// the parts of split items joined:  o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
+// ---------------------------------------------------------------------------------------
+constexpr int kJoinRows = 32;
+
+template <typename O, int kD>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PackedParams p) {
+  wait_for_launch_before();
+  if ((int)blockIdx.x >= __ldcg(&p.header->n_joins)) return;
+  const JoinEntry e = p.header->joins[blockIdx.x];
+  constexpr int kLanes = kD / 4;                 // threads of a row, four columns each
+  const int col = (threadIdx.x % kLanes) * 4;
+  for (int k = threadIdx.x / kLanes; k < kJoinRows; k += 256 / kLanes) {
+    const int row = blockIdx.y * kJoinRows + k, rr = row % kBM, tok = row / kBM * p.tpt + rr / p.group;
+    if (rr >= p.tpt * p.group || tok >= e.n_tok) continue;
+    auto part_of = [&](int w) { return w == e.w_lo ? e.part_lo : 2 * w; };
+    float top = -INFINITY;
+    for (int w = e.w_lo; w <= e.w_hi; ++w) top = fmaxf(top, p.header->part_lm[part_of(w)][row][1]);
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int w = e.w_lo; w <= e.w_hi; ++w) {
+      const int part = part_of(w);
+      const float2 lm = *reinterpret_cast<const float2*>(p.header->part_lm[part][row]);
+      const float4 x = __ldcs(reinterpret_cast<const float4*>((const char*)p.parts + (int64_t)part * kPartBytes + (row * kD + col) * 4));
+      const float f = lm.y == -INFINITY ? 0.f : ptx::ex2_approx(lm.y - top);
+      l += f * lm.x;
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    O* dst = (O*)p.o + (int64_t)(e.row0 + tok) * p.o_row + (int64_t)(e.g * p.group + rr % p.group) * p.o_head + col;
+    O y[4] = {ElemTraits<O>::from_float(acc.x * inv), ElemTraits<O>::from_float(acc.y * inv), ElemTraits<O>::from_float(acc.z * inv),
+              ElemTraits<O>::from_float(acc.w * inv)};
+    if constexpr (sizeof(O) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
   }
 }
 
@@ -909,6 +1160,14 @@ int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, packed_prefill_kernel<T, kD>, qm, km, vm, p));
+  if (!p.may_split) return G4B_OK;
+  cfg.gridDim = dim3((unsigned)workers, kPartRows / kJoinRows, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  cfg.attrs = attr + 1;
+  cfg.numAttrs = 1;
+  if (p.o_dtype == G4B_F32) G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<float, kD>, p));
+  else G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, kD>, p));
   return G4B_OK;
 }
 
@@ -949,6 +1208,7 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   if (a.k_pool.shape[3] != D) return fail(G4B_ERR_BAD_ARG, "head dim of q and pools differ");
   if (D != 256 && D != 128) return fail(G4B_ERR_UNSUPPORTED, "head dim %lld not supported (128, 256)", (long long)D);
   if (G <= 0 || H <= 0 || H % G != 0) return fail(G4B_ERR_BAD_ARG, "query heads must be a multiple of kv heads");
+  if (G > 0x7fff) return fail(G4B_ERR_UNSUPPORTED, "at most 32767 kv heads");
   if (H / G > kBM) return fail(G4B_ERR_UNSUPPORTED, "at most %d query heads per kv head", kBM);
   if (a.page_size < 16 || (a.page_size & (a.page_size - 1)) != 0) return fail(G4B_ERR_BAD_ARG, "page_size must be a power of two >= 16");
   if (a.k_pool.shape[2] != a.page_size) return fail(G4B_ERR_BAD_ARG, "pool dim 2 must equal page_size");
@@ -988,8 +1248,9 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   p.times = (const int32_t*)a.time_dim_sizes.ptr; p.time_s = a.time_dim_sizes.stride[0];
   p.block_tables = (const int32_t*)a.block_tables.ptr;
   p.bt_s0 = a.block_tables.stride[0]; p.bt_s1 = a.block_tables.stride[1];
-  p.header = (int32_t*)a.workspace.ptr;
-  p.items = (PackedItem*)((char*)a.workspace.ptr + kHeaderBytes);
+  p.header = (PackedHeader*)a.workspace.ptr;
+  p.parts = (float*)((char*)a.workspace.ptr + kPartsAt);
+  p.items = (PackedItem*)((char*)a.workspace.ptr + kItemsAt);
   p.o_row = a.o.stride[0]; p.o_head = a.o.stride[1];
   p.N = (int)N; p.B = (int)B; p.H = (int)H; p.G = (int)G;
   p.group = (int)(H / G); p.tpt = kBM / p.group;
@@ -1026,8 +1287,13 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   if (dev < 0 || dev >= 64) return fail(G4B_ERR_CUDA, "device index out of range");
   if (sm_count[dev] == 0) G4B_CUDA_CHECK(cudaDeviceGetAttribute(&sm_count[dev], cudaDevAttrMultiProcessorCount, dev));
   int64_t workers = sm_count[dev] / 2;
-  if (workers > max_items * G) workers = max_items * G;
+  if (workers > kMaxWorkers) workers = kMaxWorkers;
   if (workers < 1) workers = 1;
+  // Shares pay only where items are few (with six a worker the list of whole ones is balanced) and contexts
+  // can be long; what the contexts really are is looked at on the device.  Nor without any of that a third launch.
+  p.may_split = (N / (2 * p.tpt)) * G < 6 * workers && (int64_t)p.max_pages * a.page_size > 8 * kBN;
+  if (!p.may_split && workers > max_items * G) workers = max_items * G;
+  p.workers = (int)workers;
   if (a.k_pool.dtype == G4B_BF16)
     return D == 256 ? launch_typed<__nv_bfloat16, 256>(qm, km, vm, p, (int)workers, st) : launch_typed<__nv_bfloat16, 128>(qm, km, vm, p, (int)workers, st);
   return D == 256 ? launch_typed<__half, 256>(qm, km, vm, p, (int)workers, st) : launch_typed<__half, 128>(qm, km, vm, p, (int)workers, st);
@@ -1037,7 +1303,8 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
 
 extern "C" int64_t g4b_packed_workspace_bytes(int64_t rows, int64_t slots, int q_heads, int kv_heads) {
   if (rows < 0 || slots < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > g4b::kBM) return 0;
-  return g4b::kHeaderBytes + (int64_t)sizeof(g4b::PackedItem) * g4b::items_bound(rows, slots, q_heads / kv_heads);
+  // (every worker's boundary may add an entry)
+  return g4b::kItemsAt + (int64_t)sizeof(g4b::PackedItem) * (g4b::items_bound(rows, slots, q_heads / kv_heads) * kv_heads + 2 * g4b::kMaxWorkers);
 }
 
 extern "C" int g4b_flash_attention_packed(const G4bPackedAttnArgs* args, void* cuda_stream) {

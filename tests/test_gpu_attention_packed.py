@@ -160,6 +160,33 @@ def test_long_prompts_and_cached_contexts(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,times,kw", [
+    ([1], [30000], {}), ([1], [1025], {}), ([1, 1, 1], [5000, 1, 9000], dict(H=3, G=1)), ([5, 0, 20, 0], [9000, 0, 4000, 30], dict(D=128)),
+    ([70, 10], [3, 20000], dict(dtype=F16)), ([300], [7000], dict(out=F32)), ([200, 1], [2500, 8000], dict(D=128, out=F32, page=128)),
+    ([64] * 9, [700 * i + 64 for i in range(9)], dict(H=4, G=4, dtype=F16)), ([40, 1, 1], [6000, 1500, 16], dict(H=48, G=1, D=128)),
+    ([1] * 40 + [100], [20] * 40 + [15000], dict(H=2, G=1)), ([1100], [1100], dict(H=1, G=1))])
+def test_shares_of_long_contexts(cuda, rows, times, kw):
+    """Few items behind long contexts: their keys are cut at the workers' boundaries and the parts joined."""
+    both(make(sum(times), rows, times, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(sliding_window=3000), dict(stage=fa2.STAGE_FULL), dict(stage=fa2.STAGE_FULL, sliding_window=2500)])
+def test_shares_under_other_masks(cuda, kw):
+    both(make(31, [30, 1, 64], [7000, 12000, 64], H=4, G=2), **kw)
+
+
+@pytest.mark.gpu
+def test_shares_repeat_and_do_not_touch_other_rows(cuda):
+    c = make(32, [20, 1, 0, 7], [9000, 3000, 50, 12000])
+    both(c)
+    first = c["o"].clone()
+    for _ in range(5):
+        run(c)
+        assert torch.equal(c["o"], first)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [33, 150, 400])
 def test_many_slots(cuda, n):
     g = torch.Generator().manual_seed(n)
