@@ -38,7 +38,10 @@ namespace {
 
 constexpr int kBM = 128;           // rows per CTA: (token, head) pairs
 constexpr int kBN = 128;           // keys per S tile
-constexpr int kThreads = 352;      // producer warps 0 (Q and K) and 10 (V), MMA warp 1, 2 softmax warpgroups
+constexpr int kThreads = 384;      // 2 softmax warpgroups; producer warps 8 (Q and K) and 10 (V), MMA warp 9, one idle
+// Registers a thread: launched with 168, of which the softmax warps take from the others (2 x 128 x 200 + 128 x 104 =
+// 384 x 168)
+constexpr int kRegsSoftmax = 200, kRegsOther = 104;
 constexpr int kStageBytes = 8 * 4096;         // output: 4 KB per softmax warp
 constexpr int kXchgBytes = 2 * 2 * kBM * 4;   // row maxima: [tile parity][column half][row]
 
@@ -111,6 +114,8 @@ struct PackedParams {
   int32_t* status;
 };
 
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther)); }
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax)); }
 __device__ __forceinline__ void record(int32_t* status, int32_t code) { atomicCAS(status, 0, code); }
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -492,7 +497,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   ptx::cluster_sync_all();
   if (*reinterpret_cast<volatile int32_t*>(&bars->abort_flag) != 0) return;
 
-  if (warp == 1) {
+  if (warp == 9) {
     ptx::tmem_alloc_pair(ptx::smem_u32(&bars->tmem_base), 512);
     ptx::tmem_relinquish_pair();
   }
@@ -532,12 +537,14 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     if (lane == 0) ptx::mbar_arrive_cluster_relaxed(bar);
   };
 
-  if (warp == 0 || warp == 10) {
+  if (warp >= 8) {
+  give_registers();       // (all four warps of the group, the idle one too)
+  if (warp == 8 || warp == 10) {
     // =============================== producers ===============================
-    // Warp 0 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB, 32 of them a tile, and one
+    // Warp 8 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB, 32 of them a tile, and one
     // warp does not issue them as fast as the tensor pipe consumes them (4 prompts of 8192 rows, 8 / 2 heads,
     // pages of 16: 1153 us with one producer warp, 846 us with two).
-    const bool for_k = warp == 0, for_v = warp == 10;
+    const bool for_k = warp == 8, for_v = warp == 10;
     const uint64_t pol_kv = ptx::policy_evict_last();    // K/V tiles are re-read by every block of the slot
     const uint64_t pol_q = ptx::policy_evict_first();
     const uint32_t q_bytes = (uint32_t)(kSlabs * p.tpt * p.group * 128);
@@ -651,7 +658,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       }
       ++n_done;
     }
-  } else if (warp == 1) {
+  } else if (warp == 9) {
     // =============================== MMA issuer ===============================
     // Only CTA 0 issues.  One MMA spans both CTAs: rows 0..127 of the 256-row tile (A operand,
     // accumulator, P) are CTA 0's, rows 128..255 CTA 1's; the B operand is split between the two
@@ -760,17 +767,19 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       }
     }
     __syncwarp();
+  }
   } else {
     // =============================== softmax / epilogue ===============================
-    // Two warpgroups share every row: warps 2..5 own the first 64 keys of a tile (and the first half of
-    // O's columns), warps 6..9 the other 64.  A warp and its partner (warp + 4, same TMEM lanes) trade
+    // Two warpgroups share every row: warps 0..3 own the first 64 keys of a tile (and the first half of
+    // O's columns), warps 4..7 the other 64.  A warp and its partner (warp + 4, same TMEM lanes) trade
     // row maxima through shared memory.
-    const int half = (warp - 2) >> 2;
+    take_registers();
+    const int half = warp >> 2;
     const int lane_base = (warp & 3) * 32;
     const int r = lane_base + lane;                       // row of the tile = TMEM lane
     const uint32_t trow = tmem + ((uint32_t)lane_base << 16);
     const uint32_t pair_bar = ptx::smem_u32(&bars->pair[warp & 3]);
-    uint8_t* stage = sStage + (warp - 2) * 4096;
+    uint8_t* stage = sStage + warp * 4096;
     const int tok_r = (int)rank * p.tpt + r / p.group;    // this row's token of the block ...
     const bool in_tile = r < p.tpt * p.group;
     uint32_t pair_phase = 0;
@@ -816,9 +825,9 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       const PackedItem it = it_nx_;
       auto fetch_next = [&]() { fetch_item(item_of_round(round + 1), it_nx_); };
       if (item < 0) continue;
-      const int g = it.g_part & 0xffff;
       const int n_tiles = it.n_tiles;
       if (n_tiles <= 0) {
+        const int g = it.g_part & 0xffff;
         fetch_next();
         // no visible key for any row of the block: the output rows are zero
         *reinterpret_cast<uint4*>(stage + lane * 128) = make_uint4(0u, 0u, 0u, 0u);
@@ -1010,7 +1019,11 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       }
 
       if (!few_keys && m_used != -INFINITY) m_carry = m_used;
+      // (what the epilogue needs of the entry is read again: kept through the tile loop it costs registers there)
+      PackedItem me;
+      fetch_item(item, me);
       fetch_next();
+      const int g = me.g_part & 0xffff;
       // ---- epilogue: O / l -> global ----
       if (ok) {
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (tg + n_tiles - 1) & 1))) { record(p.status, kErrPvDone); ok = false; }
@@ -1029,12 +1042,12 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         auto put = [&](int c, uint32_t a, uint32_t b2, uint32_t c2, uint32_t d) {
           *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(a, b2, c2, d);
         };
-        const int part = it.g_part >> 16;
+        const int part = me.g_part >> 16;
         if (part > 0 || p.o_dtype == G4B_F32) {
           // f32 rows: an output of that type, or a part (un-normalised, with its sum and reference maximum in
           // log2 units; a row that saw no key here has neither)
           const float factor = part > 0 ? 1.f : inv_l;
-          if (part > 0 && half == 0 && in_tile && tok_r < it.n_tok)
+          if (part > 0 && half == 0 && in_tile && tok_r < me.n_tok)
             *reinterpret_cast<float2*>(p.header->part_lm[part - 1][(int)rank * kBM + r]) = make_float2(l_run, l_run == 0.f ? -INFINITY : m_used);
 #pragma unroll 1
           for (int c = 0; c < kHalfCols / 32; ++c) {
@@ -1045,7 +1058,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * factor);
 #pragma unroll
             for (int i = 0; i < 8; ++i) put(i, ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
-            store_stage(it, g, part, (half * kHalfCols + c * 32) * 4);
+            store_stage(me, g, part, (half * kHalfCols + c * 32) * 4);
           }
           ptx::tc_fence_before();
           arrive_issuer(issuer_bar(&bars->o_free));
@@ -1072,7 +1085,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
               const uint32_t* x = &pk[i >> 2][(i & 3) * 4];
               put(i, x[0], x[1], x[2], x[3]);
             }
-            store_stage(it, g, 0, (half * kHalfCols + c * 64) * 2);
+            store_stage(me, g, 0, (half * kHalfCols + c * 64) * 2);
           }
         }
       }
@@ -1086,7 +1099,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   __syncthreads();
   // CTA 0's MMAs read this CTA's shared and tensor memory: leave together
   ptx::cluster_sync_all();
-  if (warp == 1) {
+  if (warp == 9) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair(tmem, 512);
   }
