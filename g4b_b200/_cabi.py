@@ -279,35 +279,48 @@ _ABSENT = bytes(_VIEW.size)
 assert _VIEW.size == ctypes.sizeof(G4bTensor)
 
 
+def _view_bytes(t) -> bytes:
+    """The C view of one tensor-like that is not a torch tensor."""
+    if not (hasattr(t, "shape") and hasattr(t, "stride") and hasattr(t, "dtype") and hasattr(t, "data_ptr")):
+        raise TypeError(f"expected a tensor-like with shape/stride/dtype/data_ptr, got {type(t).__name__}")
+    _check_device(t)
+    shape, strides = [int(x) for x in t.shape], [int(x) for x in _strides(t)]
+    n = len(shape)
+    if n > 5:
+        raise ValueError("tensors of rank > 5 are not supported")
+    strides = strides[:n] + [0] * (n - len(strides))
+    pad = _PAD[5 - n]
+    return _VIEW.pack(int(t.data_ptr()), *shape, *pad, *strides, *pad, n, dtype_code(t.dtype))
+
+
 def views(*tensors) -> bytes:
     """The C views of tensor-likes (None: not given) behind one another, as bytes."""
     torch = sys.modules.get("torch")
-    current = None          # the current device, asked for once
+    if torch is None:
+        return b"".join([_ABSENT if t is None else _view_bytes(t) for t in tensors])
+    Tensor, pack, codes = torch.Tensor, _VIEW.pack, _dtype_codes
+    current = -1 if _validate_only_depth else None          # the current device, asked for once
     out = []
     for t in tensors:
         if t is None:
             out.append(_ABSENT)
-            continue
-        if torch is not None and isinstance(t, torch.Tensor):
-            if _validate_only_depth == 0:
+        elif isinstance(t, Tensor):
+            if current != -1:
                 device = t.get_device()
                 if current is None and device >= 0:
                     current = torch.cuda.current_device()
                 if device < 0 or device != current:
                     _check_device(t)
-            shape, strides = t.shape, t.stride()
+            shape = t.shape
             n = len(shape)
+            if n > 5:
+                raise ValueError("tensors of rank > 5 are not supported")
+            pad = _PAD[5 - n]
+            dt = t.dtype
+            code = codes.get(dt)
+            out.append(pack(t.data_ptr(), *shape, *pad, *t.stride(), *pad, n, dtype_code(dt) if code is None else code))
         else:
-            if not (hasattr(t, "shape") and hasattr(t, "stride") and hasattr(t, "dtype") and hasattr(t, "data_ptr")):
-                raise TypeError(f"expected a tensor-like with shape/stride/dtype/data_ptr, got {type(t).__name__}")
-            _check_device(t)
-            shape, strides = [int(x) for x in t.shape], [int(x) for x in _strides(t)]
-            n = len(shape)
-            strides = strides[:n] + [0] * (n - len(strides))
-        if n > 5:
-            raise ValueError("tensors of rank > 5 are not supported")
-        pad = _PAD[5 - n]
-        out.append(_VIEW.pack(int(t.data_ptr()), *shape, *pad, *strides, *pad, n, dtype_code(t.dtype)))
+            out.append(_view_bytes(t))
     return b"".join(out)
 
 
@@ -319,8 +332,9 @@ def as_tensor(t) -> G4bTensor:
 def current_stream(stream=None) -> int:
     """Raw cudaStream_t: an int, an object with .cuda_stream, or torch's current stream."""
     if stream is None:
-        import torch
-
+        torch = sys.modules.get("torch")
+        if torch is None:
+            import torch
         return int(torch.cuda.current_stream().cuda_stream)
     if isinstance(stream, int):
         return stream

@@ -105,6 +105,7 @@ struct PackedParams {
   int64_t o_row, o_head, starts_s, time_s, bt_s0, bt_s1;
   int N, B, H, G;
   int group, tpt;                 // query heads per kv head; tokens per CTA (kBM / group)
+  int group_mul;                  // r / group = r * group_mul >> 16 for r < kBM
   int max_items, workers;
   int may_split;                  // few enough blocks that shares can pay; then a join launch follows
   int page_shift, num_pages, max_pages;
@@ -300,6 +301,7 @@ __device__ __noinline__ void deal_shares(const PackedParams& p, int n_items) {
 // item to item, so how many items of another slot come before a given one is a closed form, and one
 // warp ranks an item with one look at every slot: no sort, no pass in between, any number of warps.
 __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ PackedParams p) {
+  wait_for_launch_before();
   let_next_launch_start();
   const int lane = threadIdx.x & 31;
   const int warp = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PackedParams p) {
   using Gm = Geo<kD>;
-  constexpr int kSt = Gm::kStages, kChunk = Gm::kChunkBytes, kSlabs = Gm::kSlabs;
+  constexpr int kSt = Gm::kStages / 2, kChunk = Gm::kChunkBytes, kSlabs = Gm::kSlabs;
   constexpr int kHalfCols = kD / 2;             // output columns of a softmax warpgroup
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -452,7 +454,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
 
   uint8_t* sQ = smem;
   uint8_t* sRing = smem + Gm::kQBytes;
-  uint8_t* sStage = sRing + kSt * kChunk;
+  uint8_t* sStage = sRing + 2 * kSt * kChunk;            // (ring: kSt chunks of K, then kSt of V)
   Barriers* bars = reinterpret_cast<Barriers*>(sStage + kStageBytes);
   float* xchg = reinterpret_cast<float*>(sStage + kStageBytes + 512);
   const uint32_t bar_q = ptx::smem_u32(&bars->q_full);
@@ -460,7 +462,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   if (threadIdx.x == 0) {
     // The barriers the MMA issuer waits on live in CTA 0 and count both CTAs.
     ptx::mbar_init(bar_q, 2);
-    for (int s = 0; s < kSt; ++s) {
+    for (int s = 0; s < 2 * kSt; ++s) {
       ptx::mbar_init(ptx::smem_u32(&bars->kv_full[s]), 2);
       ptx::mbar_init(ptx::smem_u32(&bars->kv_empty[s]), 1);
     }
@@ -544,12 +546,14 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     // Warp 8 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB, 32 of them a tile, and one
     // warp does not issue them as fast as the tensor pipe consumes them (4 prompts of 8192 rows, 8 / 2 heads,
     // pages of 16: 1153 us with one producer warp, 846 us with two).
+    // Each has its own half of the ring: with one ring the V warp, which nothing holds up at an item switch, came to a
+    // slot whose use before (a K chunk) was not even issued, and the slot's one-bit phase cannot tell that apart.
     const bool for_k = warp == 8, for_v = warp == 10;
     const uint64_t pol_kv = ptx::policy_evict_last();    // K/V tiles are re-read by every block of the slot
     const uint64_t pol_q = ptx::policy_evict_first();
     const uint32_t q_bytes = (uint32_t)(kSlabs * p.tpt * p.group * 128);
     const uint32_t bar_tail = ptx::smem_u32(&bars->tail);
-    uint32_t cc = 0;   // chunk counter over the ring (runs on across work items)
+    uint32_t cc = 0;   // chunks of this warp so far (runs on across work items)
     uint32_t tails = 0;
     int n_done = 0;
     bool ok = true;
@@ -584,16 +588,17 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         if (id < 0 || id >= p.num_pages) { record(p.status, kErrBadPage); return p.num_pages; }
         return id;
       };
+      // slot of this warp's next chunk
+      const int st_base = for_v ? kSt : 0;
       auto wait_empty = [&](int st) { return wait_lane0(ptx::smem_u32(&bars->kv_empty[st]), ((cc / kSt) & 1) ^ 1, kErrKvEmpty); };
       // K chunk = this CTA's 64 keys of the tile x kD (slabs of [64 rows x 64 d]); V chunk = all 128 keys x
       // this CTA's half of the head dim (slabs of [128 rows x 64 d]).  Lane i fetches the i-th group of
       // rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
       auto load_k = [&](int j) {
-        if (!for_k) { ++cc; return; }
         const int key0 = (it.tile_lo + j) * kBN + 64 * (int)rank + lane * p.k_rows;
         const int boxes = 64 / p.k_rows;
         const int page = lane < boxes ? page_of(key0) : 0;
-        const int st = cc % kSt;
+        const int st = st_base + cc % kSt;
         if (!wait_empty(st)) return;
         const uint32_t full = issuer_bar(&bars->kv_full[st]);
         if (lane == 0) ptx::mbar_arrive_expect_tx_cluster(full, kChunk);
@@ -608,14 +613,13 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         ++cc;
       };
       auto load_v = [&](int j) {
-        if (!for_v) { ++cc; return; }
         const int tile0 = (it.tile_lo + j) * kBN;
         const int key0 = tile0 + lane * p.v_rows;
         const int boxes = kBN / p.v_rows;
         const int page = lane < boxes ? page_of(key0) : 0;
         const int live = min(it.window - tile0, kBN);           // rows of this tile that exist
         const int dirty = live % p.v_rows;                      // the context ends inside a group
-        const int st = cc % kSt;
+        const int st = st_base + cc % kSt;
         if (!wait_empty(st)) return;
         const uint32_t full = issuer_bar(&bars->kv_full[st]);
         const uint32_t bar = dirty != 0 ? bar_tail : full;
@@ -650,11 +654,9 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         }
         ++cc;
       };
-      load_k(0);
-      if (it.n_tiles > 1 && ok) load_k(1);
       for (int j = 0; j < it.n_tiles && ok; ++j) {
-        load_v(j);
-        if (ok && j + 2 < it.n_tiles) load_k(j + 2);
+        if (for_k) load_k(j);
+        else load_v(j);
       }
       ++n_done;
     }
@@ -678,7 +680,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         ptx::tc_commit_pair(ptx::map_to_cta(a, 1));
       };
       bool ok = true;
-      uint32_t cc = 0;
+      uint32_t kc = 0, vc = 0;     // chunks of K and V so far
       int tg = 0;       // tiles issued so far: S buffer and barrier phases run on across items
       int n_done = 0;
       G4B_PACKED_LOOP_PROLOGUE();
@@ -693,8 +695,8 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         auto issue_qk = [&](int j) {
           const int t = tg + j;
           const uint32_t d_tmem = tmem + ((t & 1) ? kColS1 : kColS0);
-          const int st = cc % kSt;
-          if (!wait_all(ptx::smem_u32(&bars->kv_full[st]), (cc / kSt) & 1)) {
+          const int st = kc % kSt;
+          if (!wait_all(ptx::smem_u32(&bars->kv_full[st]), (kc / kSt) & 1)) {
             if (lane == 0) record(p.status, kErrKvFull);
             ok = false; return;
           }
@@ -712,11 +714,11 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             if (j == n_tiles - 1) commit_both(&bars->q_empty);   // last use of this item's Q
           }
           __syncwarp();
-          ++cc;
+          ++kc;
         };
         auto issue_pv = [&](int j) {
-          const int st = cc % kSt;
-          if (!wait_all(ptx::smem_u32(&bars->kv_full[st]), (cc / kSt) & 1)) {
+          const int st = kSt + vc % kSt;
+          if (!wait_all(ptx::smem_u32(&bars->kv_full[st]), (vc / kSt) & 1)) {
             if (lane == 0) record(p.status, kErrKvFull);
             ok = false; return;
           }
@@ -754,7 +756,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             }
             __syncwarp();
           }
-          ++cc;
+          ++vc;
         };
         issue_qk(0);
         if (ok && n_tiles > 1) issue_qk(1);
@@ -780,7 +782,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     const uint32_t trow = tmem + ((uint32_t)lane_base << 16);
     const uint32_t pair_bar = ptx::smem_u32(&bars->pair[warp & 3]);
     uint8_t* stage = sStage + warp * 4096;
-    const int tok_r = (int)rank * p.tpt + r / p.group;    // this row's token of the block ...
+    const int tok_r = (int)rank * p.tpt + (r * p.group_mul >> 16);    // this row's token of the block ...
     const bool in_tile = r < p.tpt * p.group;
     uint32_t pair_phase = 0;
     // bounded rendezvous of the two warps that share these rows; false when the partner never arrived
@@ -796,16 +798,20 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     const int osz = p.o_dtype == G4B_F32 ? 4 : 2;
     auto store_stage = [&](const PackedItem& it, int g, int part, int bytes0) {
       __syncwarp();
+      // rows are (token, head) pairs in this order, so those that exist are the first
+      const int rows_valid = min(it.n_tok - (int)rank * p.tpt, p.tpt) * p.group - lane_base;
+      const int c = lane & 7;
+      char* base = part > 0 ? (char*)p.parts + (int64_t)(part - 1) * kPartBytes + ((int)rank * kBM + lane_base) * (kD * 4)
+                            : (char*)p.o + ((int64_t)(it.row0 + (int)rank * p.tpt) * p.o_row + (int64_t)(g * p.group) * p.o_head) * osz;
+      base += bytes0 + c * 16;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int row = i * 4 + (lane >> 3), c = lane & 7;
-        const int rr = lane_base + row, tok = (int)rank * p.tpt + rr / p.group;
-        if (rr < p.tpt * p.group && tok < it.n_tok) {
+        const int row = i * 4 + (lane >> 3);
+        if (row < rows_valid) {
           const uint4 val = *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
-          char* dst = part > 0 ? (char*)p.parts + (int64_t)(part - 1) * kPartBytes + ((int)rank * kBM + rr) * (kD * 4)
-                               : (char*)p.o + ((int64_t)(it.row0 + tok) * p.o_row + (int64_t)(g * p.group + rr % p.group) * p.o_head) * osz;
-          dst += bytes0 + c * 16;
-          *reinterpret_cast<uint4*>(dst) = val;
+          const int tok = (lane_base + row) * p.group_mul >> 16, head = lane_base + row - tok * p.group;
+          const int64_t off = part > 0 ? (int64_t)row * (kD * 4) : (tok * p.o_row + head * p.o_head) * osz;
+          *reinterpret_cast<uint4*>(base + off) = val;
         }
       }
       __syncwarp();
@@ -944,13 +950,14 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
           }
           ptx::tmem_st16(trow + s_col + half * 32 + 16, pk + 16);
           l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+          // keep the PV-done phase bookkeeping in step (no stall: PV(j-1) ended long ago); before P(j) is handed over,
+          // since a warp held up behind that could find PV(j) done too and its one-bit phase as it was
+          if (j > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (t - 1) & 1))) {
+            record(p.status, kErrPvDone); ok = false; break;
+          }
           ptx::tc_wait_st();
           ptx::tc_fence_before();
           arrive_issuer(bar_pb);
-          // keep the PV-done phase bookkeeping in step (no stall: PV(j-1) ended long ago)
-          if (j > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (t - 1) & 1))) {
-            record(p.status, kErrPvDone); ok = false;
-          }
           continue;
         }
 
@@ -1155,29 +1162,30 @@ int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap
     G4B_CUDA_CHECK(cudaFuncSetAttribute(packed_prefill_kernel<T, kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<kD>::kSmemBytes));
     attr_set[dev] = true;
   }
-  plan_kernel<<<(unsigned)((p.max_items + 7) / 8), 256, 0, st>>>(p);
-  G4B_CUDA_CHECK(cudaGetLastError());
-  // the attention launch sets itself up while the list is being written
+  // Each launch is set up while the one before it drains (and waits for it before it reads anything).
   cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)((p.max_items + 7) / 8), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, plan_kernel, p));
   cfg.gridDim = dim3((unsigned)(2 * workers), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = Geo<kD>::kSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 2;
   G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, packed_prefill_kernel<T, kD>, qm, km, vm, p));
   if (!p.may_split) return G4B_OK;
   cfg.gridDim = dim3((unsigned)workers, kPartRows / kJoinRows, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  cfg.attrs = attr + 1;
   cfg.numAttrs = 1;
   if (p.o_dtype == G4B_F32) G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<float, kD>, p));
   else G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, kD>, p));
@@ -1267,6 +1275,7 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   p.o_row = a.o.stride[0]; p.o_head = a.o.stride[1];
   p.N = (int)N; p.B = (int)B; p.H = (int)H; p.G = (int)G;
   p.group = (int)(H / G); p.tpt = kBM / p.group;
+  p.group_mul = (65536 + p.group - 1) / p.group;
   p.max_items = (int)max_items;
   while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
   p.num_pages = (int)a.k_pool.shape[0]; p.max_pages = (int)a.block_tables.shape[1];

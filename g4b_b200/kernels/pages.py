@@ -18,22 +18,19 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status
     word says so), so what it does never depends on the order of the blocks.  Returns None."""
-    # (the pools are dozens: of each is asked what costs least)
+    # (the pools are dozens: what is asked of each is what costs least)
     pools = list(pools)
-    num_pages = int(pools[0].shape[0]) if pools and pools[0].dim() else 0
-    flat = []
-    device = None
-    for p in pools:
-        if p.get_device() != device:
-            _cabi._check_device(p)
-            device = p.get_device()
-        if not p.is_contiguous():
-            raise ValueError("page pools must be contiguous")
-        shape = p.shape
-        if not shape or shape[0] != num_pages:
-            raise ValueError("page pools must all have the same number of pages (dim 0)")
-        flat += (p.data_ptr(), p.nbytes)
-    flat[1::2] = [n // max(num_pages, 1) for n in flat[1::2]]
+    shapes = [p.shape for p in pools]
+    num_pages = shapes[0][0] if pools and shapes[0] else 0
+    for device in {p.get_device() for p in pools}:
+        _cabi._check_device(next(p for p in pools if p.get_device() == device))
+    if not all([p.is_contiguous() for p in pools]):
+        raise ValueError("page pools must be contiguous")
+    if [s for s in shapes if not s or s[0] != num_pages]:
+        raise ValueError("page pools must all have the same number of pages (dim 0)")
+    flat = [0] * (2 * len(pools))
+    flat[::2] = [p.data_ptr() for p in pools]
+    flat[1::2] = [p.nbytes // num_pages for p in pools] if num_pages else [0] * len(pools)
     table = (_cabi.G4bPagePool * len(pools)).from_buffer_copy(struct.pack(f"@{len(flat)}q", *flat))
     a = _cabi.G4bPageCopyArgs(table, num_pages)
     a.src_pages = _cabi.as_tensor(src_pages)

@@ -349,6 +349,25 @@ def test_captured_with_other_lengths_on_another_stream(cuda):
 
 
 @pytest.mark.gpu
+def test_many_calls_behind_one_another(cuda):
+    """Nothing waits between the calls: each launch is set up while the one before drains, with the same workspace."""
+    cases = [make(40, [2500, 700, 1], H=8, G=2), make(41, [5, 17], H=8, G=2), make(42, [64, 1], [9000, 4000], H=8, G=2, dtype=F16),
+             make(43, [900, 333, 41], H=8, G=2, D=128, page=64)]
+    workspace = max((c["workspace"] for c in cases), key=lambda w: w.numel())
+    want = []
+    for c in cases:
+        c["workspace"] = workspace
+        run(c, sliding_window=300 if c is cases[0] else None)
+        want.append(c["o"].clone())
+    for i in range(400):
+        c = cases[i * 7 % 4]
+        run(c, sliding_window=300 if c is cases[0] else None)
+    for c, w in zip(cases, want):
+        assert torch.equal(c["o"], w) or bool(((c["o"] - w).abs().float() <= 2e-2 * w.abs().float() + 4e-3).all())
+    assert _cabi.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_two_streams_with_their_own_workspaces(cuda):
     cases = [make(26, [900, 300], H=4, G=1), make(27, [64, 700, 1], [64, 700, 2000], H=4, G=1)]
     before = [c["o"].clone() for c in cases]
