@@ -335,7 +335,8 @@ def current_stream(stream=None) -> int:
         torch = sys.modules.get("torch")
         if torch is None:
             import torch
-        return int(torch.cuda.current_stream().cuda_stream)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (without the Stream object: 0.1 us instead of 3.3)
+        return int(raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream)
     if isinstance(stream, int):
         return stream
     for attr in ("cuda_stream", "handle"):

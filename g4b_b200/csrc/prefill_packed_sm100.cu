@@ -110,6 +110,7 @@ struct PackedParams {
   int may_split;                  // few enough blocks that shares can pay; then a join launch follows
   int page_shift, num_pages, max_pages;
   int k_rows, v_rows;             // rows of a K / V box
+  int o_boxes;                    // the output goes out by TMA: 32 (token, head) rows are a box
   int sliding_window, causal, o_dtype;
   float scale_log2;
   int32_t* status;
@@ -443,7 +444,8 @@ template <> struct PackT<__half> {
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PackedParams p) {
+                      const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
+                      const __grid_constant__ PackedParams p) {
   using Gm = Geo<kD>;
   constexpr int kSt = Gm::kStages / 2, kChunk = Gm::kChunkBytes, kSlabs = Gm::kSlabs;
   constexpr int kHalfCols = kD / 2;             // output columns of a softmax warpgroup
@@ -793,13 +795,31 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       ++pair_phase;
       return w;
     };
-    // Stores 32 rows x 128 bytes out of this warp's stage: eight lanes a row, so that a row piece is one
-    // whole line.  `bytes0`: offset of the piece inside an output row.
+    // Stores 32 rows x 128 bytes out of this warp's stage.  `bytes0`: offset of the piece inside an output row.
+    // Rows that all exist leave as one TMA box, which the copy engine reads while the warp moves on (64 KB
+    // an item, stored by the warps themselves, cost them 3500 cycles of an item's 20000 under a window of 512 keys);
+    // otherwise eight lanes store a row, so that a row piece is one whole line.
+    const uint64_t pol_o = ptx::policy_evict_first();    // the output is not read again here
+    auto stage_free = [&]() {
+      if (lane == 0) ptx::bulk_wait_read_all();
+      __syncwarp();
+    };
     const int osz = p.o_dtype == G4B_F32 ? 4 : 2;
     auto store_stage = [&](const PackedItem& it, int g, int part, int bytes0) {
-      __syncwarp();
       // rows are (token, head) pairs in this order, so those that exist are the first
       const int rows_valid = min(it.n_tok - (int)rank * p.tpt, p.tpt) * p.group - lane_base;
+      if (p.o_boxes && part == 0 && rows_valid >= 32) {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int tok = lane_base * p.group_mul >> 16;
+          ptx::tma_store_3d_hint(&o_map, ptx::smem_u32(stage), bytes0 >> 1, g * p.group + lane_base - tok * p.group,
+                                 it.row0 + (int)rank * p.tpt + tok, pol_o);
+          ptx::bulk_commit();
+        }
+        return;
+      }
+      __syncwarp();
       const int c = lane & 7;
       char* base = part > 0 ? (char*)p.parts + (int64_t)(part - 1) * kPartBytes + ((int)rank * kBM + lane_base) * (kD * 4)
                             : (char*)p.o + ((int64_t)(it.row0 + (int)rank * p.tpt) * p.o_row + (int64_t)(g * p.group) * p.o_head) * osz;
@@ -836,8 +856,8 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const int g = it.g_part & 0xffff;
         fetch_next();
         // no visible key for any row of the block: the output rows are zero
-        *reinterpret_cast<uint4*>(stage + lane * 128) = make_uint4(0u, 0u, 0u, 0u);
-        for (int c = 1; c < 8; ++c) *reinterpret_cast<uint4*>(stage + lane * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        stage_free();
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(stage + lane * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
         for (int c = 0; c < kHalfCols * osz / 128; ++c) store_stage(it, g, 0, half * kHalfCols * osz + c * 128);
         continue;
       }
@@ -861,14 +881,14 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
           record(p.status, kErrSFull); ok = false; break;
         }
         ptx::tc_fence_after();
+        uint32_t sraw[2][32];       // this thread's half of a row of scores
+        ptx::tmem_ld32(trow + s_col + half * 64, sraw[0]);
+        ptx::tmem_ld32(trow + s_col + half * 64 + 32, sraw[1]);
+        ptx::tc_wait_ld32x2(sraw[0], sraw[1]);
         const int kbase = (it.tile_lo + j) * kBN;
         // warp-uniform: does any row of this CTA need element masks in this tile?
         const bool need_mask = (p.causal && kbase + kBN - 1 > qpos_min) || (kbase + kBN > window) || (kbase < key_lo) ||
                                (p.sliding_window > 0 && kbase < qpos_max - p.sliding_window + 1);
-        uint32_t sraw[2][32];
-        ptx::tmem_ld32(trow + s_col + half * 64, sraw[0]);
-        ptx::tmem_ld32(trow + s_col + half * 64 + 32, sraw[1]);
-        ptx::tc_wait_ld();
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if (need_mask) {
           // the keys this row sees are one range [nlo, nhi) of the thread's 64: one bit per key
@@ -880,19 +900,14 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             const uint32_t below_lo = lo >= 32 ? 0xffffffffu : ((1u << lo) - 1u);
             const uint32_t bits = below_hi & ~below_lo;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float x = __uint_as_float(sraw[q2][i]);
-              x = (bits & (1u << i)) ? x : -INFINITY;
-              sraw[q2][i] = __float_as_uint(x);
-              mx4[i & 3] = fmaxf(mx4[i & 3], x);
-            }
+            for (int i = 0; i < 32; ++i) sraw[q2][i] = (bits & (1u << i)) ? sraw[q2][i] : 0xff800000u;
           }
-        } else {
-#pragma unroll
-          for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sraw[q2][i]));
         }
+#pragma unroll
+        for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            mx4[(i >> 1) & 3] = ptx::max3(mx4[(i >> 1) & 3], __uint_as_float(sraw[q2][i]), __uint_as_float(sraw[q2][i + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         // publish the half-row maximum for the partner warp; collect the partner's later.  The buffers
         // alternate with every rendezvous of the pair, so a write cannot overtake the partner's read
@@ -907,16 +922,20 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         // Optimistic path: the reference maximum rarely moves (it only has to stay within 2^8 of the
         // true one), so start exponentiating against the current one while the maxima are traded.
         bool fast = !few_keys && __all_sync(0xffffffffu, m_used != -INFINITY);
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-        if (fast) {
-          const float neg_m = -m_used;
+        float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto weights = [&](const uint32_t (&x)[32], float neg_m, uint32_t* out) {
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float p0 = ptx::ex2_approx(fmaf(__uint_as_float(sraw[0][i]), p.scale_log2, neg_m));
-            const float p1 = ptx::ex2_approx(fmaf(__uint_as_float(sraw[0][i + 1]), p.scale_log2, neg_m));
-            sum4[(i >> 1) & 3] += p0 + p1;
-            pk[i >> 1] = PackT<T>::pack(p0, p1);
+            const float2 e = ptx::fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
+                                       make_float2(p.scale_log2, p.scale_log2), make_float2(neg_m, neg_m));
+            const float2 w = make_float2(ptx::ex2_approx(e.x), ptx::ex2_approx(e.y));
+            sum2[(i >> 1) & 1] = ptx::add2(sum2[(i >> 1) & 1], w);
+            out[i >> 1] = PackT<T>::pack(w.x, w.y);
           }
+        };
+        if (fast) {
+          const float neg_m = -m_used;
+          weights(sraw[0], neg_m, pk);
         }
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(pair_bar, pair_phase & 1))) {
           record(p.status, kErrPair); ok = false; break;
@@ -941,15 +960,9 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
           ptx::tc_fence_before();
           arrive_issuer(bar_pa);
           const float neg_m = -m_used;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ptx::ex2_approx(fmaf(__uint_as_float(sraw[1][i]), p.scale_log2, neg_m));
-            const float p1 = ptx::ex2_approx(fmaf(__uint_as_float(sraw[1][i + 1]), p.scale_log2, neg_m));
-            sum4[(i >> 1) & 3] += p0 + p1;
-            pk[16 + (i >> 1)] = PackT<T>::pack(p0, p1);
-          }
+          weights(sraw[1], neg_m, pk + 16);
           ptx::tmem_st16(trow + s_col + half * 32 + 16, pk + 16);
-          l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+          l_run += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
           // keep the PV-done phase bookkeeping in step (no stall: PV(j-1) ended long ago); before P(j) is handed over,
           // since a warp held up behind that could find PV(j) done too and its one-bit phase as it was
           if (j > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (t - 1) & 1))) {
@@ -973,7 +986,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         }
         l_run *= alpha;
         const float neg_m = (m_used == -INFINITY) ? 0.f : -m_used;
-        sum4[0] = sum4[1] = sum4[2] = sum4[3] = 0.f;
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
         // O may only be touched once PV(j-1) has drained, and must be rescaled before any part of P(j) is
         // published
         if (j > 0) {
@@ -1063,6 +1076,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             ptx::tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * factor);
+            stage_free();
 #pragma unroll
             for (int i = 0; i < 8; ++i) put(i, ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
             store_stage(me, g, part, (half * kHalfCols + c * 32) * 4);
@@ -1087,6 +1101,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
               ptx::tc_fence_before();
               arrive_issuer(issuer_bar(&bars->o_free));
             }
+            stage_free();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const uint32_t* x = &pk[i >> 2][(i & 3) * 4];
@@ -1102,6 +1117,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   }
 
   // ---- teardown: every thread arrives here, on success and after a failed wait ----
+  if (warp < 8 && lane == 0) ptx::bulk_wait_all();   // the output boxes handed to the copy engine are stored
   ptx::tc_fence_before();
   __syncthreads();
   // CTA 0's MMAs read this CTA's shared and tensor memory: leave together
@@ -1154,7 +1170,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Packe
 // host side
 // ---------------------------------------------------------------------------------------
 template <typename T, int kD>
-int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PackedParams& p, int workers, cudaStream_t st) {
+int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& om, const PackedParams& p, int workers, cudaStream_t st) {
   static bool attr_set[64] = {false};
   int dev = 0;
   G4B_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1181,7 +1197,7 @@ int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = Geo<kD>::kSmemBytes;
   cfg.numAttrs = 2;
-  G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, packed_prefill_kernel<T, kD>, qm, km, vm, p));
+  G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, packed_prefill_kernel<T, kD>, qm, km, vm, om, p));
   if (!p.may_split) return G4B_OK;
   cfg.gridDim = dim3((unsigned)workers, kPartRows / kJoinRows, 1);
   cfg.blockDim = dim3(256, 1, 1);
@@ -1303,6 +1319,19 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
     if ((rc = encode_map(&km, a.k_pool.dtype, 4, a.k_pool.ptr, pdims, pstr, kbox, "k_pool"))) return rc;
     if ((rc = encode_map(&vm, a.v_pool.dtype, 4, a.v_pool.ptr, pdims, pstr, vbox, "v_pool"))) return rc;
   }
+  // The output as boxes of the 32 rows that a warp holds: 32 / (heads of a group) tokens, or 32 heads of one.  Other
+  // group sizes, f32, and layouts that a descriptor cannot express (the driver refuses it) are stored by the warps.
+  CUtensorMap om = qm;
+  if ((p.group & (p.group - 1)) == 0 && a.o.dtype != G4B_F32) {
+    const uint64_t head = H > 1 ? (uint64_t)a.o.stride[1] * esz : (uint64_t)D * esz;
+    const uint64_t row = N > 1 ? (uint64_t)a.o.stride[0] * esz : (uint64_t)(H * D) * esz;
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)H, (uint64_t)N};
+    const uint64_t strides[2] = {head, row};
+    const uint32_t gw = p.group < 32 ? (uint32_t)p.group : 32u;
+    const uint32_t box[3] = {64, gw, 32 / gw};
+    p.o_boxes = encode_map(&om, a.o.dtype, 3, a.o.ptr, dims, strides, box, "o") == G4B_OK;
+    if (!p.o_boxes) om = qm;
+  }
   static int sm_count[64] = {0};
   int dev = 0;
   G4B_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1317,8 +1346,8 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   if (!p.may_split && workers > max_items * G) workers = max_items * G;
   p.workers = (int)workers;
   if (a.k_pool.dtype == G4B_BF16)
-    return D == 256 ? launch_typed<__nv_bfloat16, 256>(qm, km, vm, p, (int)workers, st) : launch_typed<__nv_bfloat16, 128>(qm, km, vm, p, (int)workers, st);
-  return D == 256 ? launch_typed<__half, 256>(qm, km, vm, p, (int)workers, st) : launch_typed<__half, 128>(qm, km, vm, p, (int)workers, st);
+    return D == 256 ? launch_typed<__nv_bfloat16, 256>(qm, km, vm, om, p, (int)workers, st) : launch_typed<__nv_bfloat16, 128>(qm, km, vm, om, p, (int)workers, st);
+  return D == 256 ? launch_typed<__half, 256>(qm, km, vm, om, p, (int)workers, st) : launch_typed<__half, 128>(qm, km, vm, om, p, (int)workers, st);
 }
 
 }  // namespace g4b

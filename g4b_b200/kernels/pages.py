@@ -30,7 +30,7 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
         raise ValueError("page pools must all have the same number of pages (dim 0)")
     flat = [0] * (2 * len(pools))
     flat[::2] = [p.data_ptr() for p in pools]
-    flat[1::2] = [p.nbytes // num_pages for p in pools] if num_pages else [0] * len(pools)
+    flat[1::2] = [p.nbytes for p in pools] if num_pages < 2 else [p.nbytes // num_pages for p in pools]
     table = (_cabi.G4bPagePool * len(pools)).from_buffer_copy(struct.pack(f"@{len(flat)}q", *flat))
     a = _cabi.G4bPageCopyArgs(table, num_pages)
     a.src_pages = _cabi.as_tensor(src_pages)
