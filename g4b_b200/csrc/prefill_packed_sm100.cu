@@ -1131,38 +1131,50 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
 // ---------------------------------------------------------------------------------------
 // the parts of split items joined:  o = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
 // ---------------------------------------------------------------------------------------
-constexpr int kJoinRows = 32;
+// A warp takes one (item, row): few CTAs, so that a call that split nothing pays little for this launch, and every
+// warp with the loads of several parts in flight.
+constexpr int kJoinWarps = 16, kJoinBlocks = 296;
 
 template <typename O, int kD>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PackedParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PackedParams p) {
   wait_for_launch_before();
-  if ((int)blockIdx.x >= __ldcg(&p.header->n_joins)) return;
-  const JoinEntry e = p.header->joins[blockIdx.x];
-  constexpr int kLanes = kD / 4;                 // threads of a row, four columns each
-  const int col = (threadIdx.x % kLanes) * 4;
-  for (int k = threadIdx.x / kLanes; k < kJoinRows; k += 256 / kLanes) {
-    const int row = blockIdx.y * kJoinRows + k, rr = row % kBM, tok = row / kBM * p.tpt + rr / p.group;
+  const int n_rows = __ldcg(&p.header->n_joins) * kPartRows;
+  const int lane = threadIdx.x & 31;
+  constexpr int kVecs = kD / 128;                // float4 of a lane
+  for (int u = blockIdx.x * kJoinWarps + (threadIdx.x >> 5); u < n_rows; u += kJoinBlocks * kJoinWarps) {
+    const JoinEntry e = p.header->joins[u / kPartRows];
+    const int row = u % kPartRows, rr = row % kBM, tok_c = rr * p.group_mul >> 16, tok = row / kBM * p.tpt + tok_c;
     if (rr >= p.tpt * p.group || tok >= e.n_tok) continue;
     auto part_of = [&](int w) { return w == e.w_lo ? e.part_lo : 2 * w; };
     float top = -INFINITY;
-    for (int w = e.w_lo; w <= e.w_hi; ++w) top = fmaxf(top, p.header->part_lm[part_of(w)][row][1]);
+    for (int w = e.w_lo + lane; w <= e.w_hi; w += 32) top = fmaxf(top, p.header->part_lm[part_of(w)][row][1]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 acc[kVecs];
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int w = e.w_lo; w <= e.w_hi; ++w) {
       const int part = part_of(w);
       const float2 lm = *reinterpret_cast<const float2*>(p.header->part_lm[part][row]);
-      const float4 x = __ldcs(reinterpret_cast<const float4*>((const char*)p.parts + (int64_t)part * kPartBytes + (row * kD + col) * 4));
       const float f = lm.y == -INFINITY ? 0.f : ptx::ex2_approx(lm.y - top);
       l += f * lm.x;
-      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>((const char*)p.parts + (int64_t)part * kPartBytes + (row * kD + v * 128 + lane * 4) * 4));
+        acc[v].x += f * x.x; acc[v].y += f * x.y; acc[v].z += f * x.z; acc[v].w += f * x.w;
+      }
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    O* dst = (O*)p.o + (int64_t)(e.row0 + tok) * p.o_row + (int64_t)(e.g * p.group + rr % p.group) * p.o_head + col;
-    O y[4] = {ElemTraits<O>::from_float(acc.x * inv), ElemTraits<O>::from_float(acc.y * inv), ElemTraits<O>::from_float(acc.z * inv),
-              ElemTraits<O>::from_float(acc.w * inv)};
-    if constexpr (sizeof(O) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
-    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      O* dst = (O*)p.o + (int64_t)(e.row0 + tok) * p.o_row + (int64_t)(e.g * p.group + rr - tok_c * p.group) * p.o_head + v * 128 + lane * 4;
+      O y[4] = {ElemTraits<O>::from_float(acc[v].x * inv), ElemTraits<O>::from_float(acc[v].y * inv), ElemTraits<O>::from_float(acc[v].z * inv),
+                ElemTraits<O>::from_float(acc[v].w * inv)};
+      if constexpr (sizeof(O) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(y);
+      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+    }
   }
 }
 
@@ -1199,8 +1211,8 @@ int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap
   cfg.numAttrs = 2;
   G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, packed_prefill_kernel<T, kD>, qm, km, vm, om, p));
   if (!p.may_split) return G4B_OK;
-  cfg.gridDim = dim3((unsigned)workers, kPartRows / kJoinRows, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.gridDim = dim3(kJoinBlocks, 1, 1);
+  cfg.blockDim = dim3(kJoinWarps * 32, 1, 1);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   if (p.o_dtype == G4B_F32) G4B_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<float, kD>, p));

@@ -176,7 +176,7 @@ __device__ __forceinline__ void rows_of_kind(const RopePackedParams& p, int h_be
 }
 
 template <typename In, int kLanes, int kIters, bool kExact, int kOut>
-__global__ void __launch_bounds__(32, kIters == 1 ? 28 : 16) rope_packed_kernel(const __grid_constant__ RopePackedParams p) {
+__global__ void __launch_bounds__(32, kIters == 1 ? 32 : 16) rope_packed_kernel(const __grid_constant__ RopePackedParams p) {
   const int lane = threadIdx.x;
   const int row = (int)(p.n_slots == 1 ? blockIdx.x : blockIdx.x / p.n_slots);
   const int part = (int)(blockIdx.x - (uint32_t)row * p.n_slots);
