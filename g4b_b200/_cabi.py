@@ -274,7 +274,7 @@ def _check_device(t) -> None:
 # a G4bTensor as bytes: pointer, 5 extents, 5 strides, rank, dtype.  Packed in one go: field by
 # field a view costs three times as much, and a call packs a dozen.
 _VIEW = struct.Struct("@P5q5qii")
-_PAD = [(0,) * i for i in range(6)]
+_VIEW_OF_RANK = [struct.Struct(f"@P{n}q{8 * (5 - n)}x{n}q{8 * (5 - n)}xii") for n in range(6)]     # (pad bytes are zeros)
 _ABSENT = bytes(_VIEW.size)
 assert _VIEW.size == ctypes.sizeof(G4bTensor)
 
@@ -289,8 +289,7 @@ def _view_bytes(t) -> bytes:
     if n > 5:
         raise ValueError("tensors of rank > 5 are not supported")
     strides = strides[:n] + [0] * (n - len(strides))
-    pad = _PAD[5 - n]
-    return _VIEW.pack(int(t.data_ptr()), *shape, *pad, *strides, *pad, n, dtype_code(t.dtype))
+    return _VIEW_OF_RANK[n].pack(int(t.data_ptr()), *shape, *strides, n, dtype_code(t.dtype))
 
 
 def views(*tensors) -> bytes:
@@ -298,7 +297,7 @@ def views(*tensors) -> bytes:
     torch = sys.modules.get("torch")
     if torch is None:
         return b"".join([_ABSENT if t is None else _view_bytes(t) for t in tensors])
-    Tensor, pack, codes = torch.Tensor, _VIEW.pack, _dtype_codes
+    Tensor, packers, codes = torch.Tensor, _VIEW_OF_RANK, _dtype_codes
     current = -1 if _validate_only_depth else None          # the current device, asked for once
     out = []
     for t in tensors:
@@ -307,18 +306,17 @@ def views(*tensors) -> bytes:
         elif isinstance(t, Tensor):
             if current != -1:
                 device = t.get_device()
-                if current is None and device >= 0:
-                    current = torch.cuda.current_device()
-                if device < 0 or device != current:
-                    _check_device(t)
+                if device != current:
+                    if current is None and device >= 0:
+                        current = torch.cuda.current_device()
+                    if device != current:
+                        _check_device(t)
             shape = t.shape
             n = len(shape)
             if n > 5:
                 raise ValueError("tensors of rank > 5 are not supported")
-            pad = _PAD[5 - n]
-            dt = t.dtype
-            code = codes.get(dt)
-            out.append(pack(t.data_ptr(), *shape, *pad, *t.stride(), *pad, n, dtype_code(dt) if code is None else code))
+            code = codes.get(t.dtype)
+            out.append(packers[n].pack(t.data_ptr(), *shape, *t.stride(), n, dtype_code(t.dtype) if code is None else code))
         else:
             out.append(_view_bytes(t))
     return b"".join(out)

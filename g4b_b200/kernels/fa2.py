@@ -217,5 +217,5 @@ def flash_attention_packed(q, k_pool, v_pool, o, q_starts, time_dim_sizes, *, bl
     a = _cabi.G4bPackedAttnArgs.from_buffer_copy(
         _cabi.views(q, o, k_pool, v_pool, q_starts, time_dim_sizes, block_tables, workspace)
         + _PACKED_TAIL.pack(page_size, stage, sliding_window or 0, scale))
-    _cabi.check(_cabi.load().g4b_flash_attention_packed(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
+    _cabi.check(_cabi.load().g4b_flash_attention_packed(ctypes.byref(a), _cabi.current_stream(stream)))
     return None

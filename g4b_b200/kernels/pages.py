@@ -8,6 +8,8 @@ import struct
 
 from g4b_b200 import _cabi
 
+_HEAD, _TAIL = struct.Struct("@Pq"), struct.Struct("@ii")      # G4bPageCopyArgs around its two views
+
 
 def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     """``pool[dst_pages[i]] = pool[src_pages[i]]`` in every pool of ``pools``, in one launch
@@ -18,7 +20,7 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status
     word says so), so what it does never depends on the order of the blocks.  Returns None."""
-    # (the pools are dozens: what is asked of each is what costs least)
+    # (the pools are dozens: each thing is asked of all of them at once, the cheapest way)
     pools = list(pools)
     shapes = [p.shape for p in pools]
     num_pages = shapes[0][0] if pools and shapes[0] else 0
@@ -30,11 +32,11 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
         raise ValueError("page pools must all have the same number of pages (dim 0)")
     flat = [0] * (2 * len(pools))
     flat[::2] = [p.data_ptr() for p in pools]
-    flat[1::2] = [p.nbytes for p in pools] if num_pages < 2 else [p.nbytes // num_pages for p in pools]
-    table = (_cabi.G4bPagePool * len(pools)).from_buffer_copy(struct.pack(f"@{len(flat)}q", *flat))
-    a = _cabi.G4bPageCopyArgs(table, num_pages)
-    a.src_pages = _cabi.as_tensor(src_pages)
-    a.dst_pages = _cabi.as_tensor(dst_pages)
-    a.num_pools = len(pools)
-    _cabi.check(_cabi.load().g4b_page_copy(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
+    if num_pages:
+        flat[1::2] = [p.nbytes // num_pages for p in pools]
+    a = _cabi.G4bPageCopyArgs.from_buffer_copy(
+        _HEAD.pack(0, num_pages) + _cabi.views(src_pages, dst_pages) + _TAIL.pack(len(pools), 0))
+    table = struct.pack(f"@{len(flat)}q", *flat)
+    a.pools = ctypes.cast(ctypes.c_char_p(table), ctypes.POINTER(_cabi.G4bPagePool))
+    _cabi.check(_cabi.load().g4b_page_copy(ctypes.byref(a), _cabi.current_stream(stream)))
     return None

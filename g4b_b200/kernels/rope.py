@@ -139,9 +139,9 @@ def rope_norm_append_packed(
         _cabi.views(q, k, v, q_out, rope_freqs, positions, pair_axis, q_starts, time_dim_sizes, q_rmsnorm_w, k_rmsnorm_w,
                     k_pool, v_pool, block_tables)
         + _PACKED_TAIL.pack(rmsnorm_eps, page_size, 1 if norm_qk else 0, 1 if norm_v else 0))
-    if a.positions.ndim == 1:            # one axis
+    if positions is not None and len(positions.shape) == 1:            # one axis
         n, step = a.positions.shape[0], a.positions.stride[0]
         a.positions.ndim, a.positions.shape[0], a.positions.stride[0] = 2, 1, 0
         a.positions.shape[1], a.positions.stride[1] = n, step
-    _cabi.check(_cabi.load().g4b_rope_norm_append_packed(ctypes.byref(a), ctypes.c_void_p(_cabi.current_stream(stream))))
+    _cabi.check(_cabi.load().g4b_rope_norm_append_packed(ctypes.byref(a), _cabi.current_stream(stream)))
     return None
