@@ -499,7 +499,10 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     ptx::fence_proxy_async_smem();
   }
   ptx::cluster_sync_all();
-  if (*reinterpret_cast<volatile int32_t*>(&bars->abort_flag) != 0) return;
+  if (*reinterpret_cast<volatile int32_t*>(&bars->abort_flag) != 0) {
+    wait_for_launch_before();           // (what follows this launch may rely on the one before it being done)
+    return;
+  }
 
   if (warp == 9) {
     ptx::tmem_alloc_pair(ptx::smem_u32(&bars->tmem_base), 512);
@@ -581,10 +584,11 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         for (int s = 0; s < kSlabs; ++s)
           ptx::tma_load_3d_pair(ptx::smem_u32(sQ + s * 16384), &q_map, qb, s * 64, g * p.group, it.row0 + (int)rank * p.tpt, pol_q);
       }
-      // page of the group of rows that starts at `key`; num_pages (outside the pool: zero fill) for groups
-      // past the context and for bad entries
-      auto page_of = [&](int key) -> int {
-        if (key >= it.window) return p.num_pages;
+      // page of the group of `rows` keys that starts at `key`; num_pages (outside the pool: zero fill) for groups past
+      // the context, in front of every row's window (their pages may be gone) and for bad entries
+      const int first_key = p.sliding_window > 0 ? it.qpos0 - p.sliding_window + 1 : 0;
+      auto page_of = [&](int key, int rows) -> int {
+        if (key >= it.window || key + rows <= first_key) return p.num_pages;
         const int pg = key >> p.page_shift;          // (< max_pages: the window is bounded by the table)
         const int id = bt[pg * p.bt_s1];
         if (id < 0 || id >= p.num_pages) { record(p.status, kErrBadPage); return p.num_pages; }
@@ -599,7 +603,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       auto load_k = [&](int j) {
         const int key0 = (it.tile_lo + j) * kBN + 64 * (int)rank + lane * p.k_rows;
         const int boxes = 64 / p.k_rows;
-        const int page = lane < boxes ? page_of(key0) : 0;
+        const int page = lane < boxes ? page_of(key0, p.k_rows) : 0;
         const int st = st_base + cc % kSt;
         if (!wait_empty(st)) return;
         const uint32_t full = issuer_bar(&bars->kv_full[st]);
@@ -618,7 +622,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const int tile0 = (it.tile_lo + j) * kBN;
         const int key0 = tile0 + lane * p.v_rows;
         const int boxes = kBN / p.v_rows;
-        const int page = lane < boxes ? page_of(key0) : 0;
+        const int page = lane < boxes ? page_of(key0, p.v_rows) : 0;
         const int live = min(it.window - tile0, kBN);           // rows of this tile that exist
         const int dirty = live % p.v_rows;                      // the context ends inside a group
         const int st = st_base + cc % kSt;
@@ -1138,6 +1142,8 @@ constexpr int kJoinWarps = 16, kJoinBlocks = 296;
 template <typename O, int kD>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PackedParams p) {
   wait_for_launch_before();
+  const int32_t status = __ldcg(p.status);
+  if ((status & 0xf00) == 0x300 && status != kErrBadPage) return;      // the parts are not complete
   const int n_rows = __ldcg(&p.header->n_joins) * kPartRows;
   const int lane = threadIdx.x & 31;
   constexpr int kVecs = kD / 128;                // float4 of a lane
@@ -1187,6 +1193,10 @@ int launch_typed(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap
   int dev = 0;
   G4B_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+    // (the registers that the softmax warps take must be there, or they wait for ever)
+    cudaFuncAttributes fa;
+    G4B_CUDA_CHECK(cudaFuncGetAttributes(&fa, packed_prefill_kernel<T, kD>));
+    if (fa.numRegs * kThreads < 256 * kRegsSoftmax + 128 * kRegsOther) return fail(G4B_ERR_CUDA, "packed attention was built with %d registers a thread", fa.numRegs);
     G4B_CUDA_CHECK(cudaFuncSetAttribute(packed_prefill_kernel<T, kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<kD>::kSmemBytes));
     attr_set[dev] = true;
   }
@@ -1309,7 +1319,8 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   p.num_pages = (int)a.k_pool.shape[0]; p.max_pages = (int)a.block_tables.shape[1];
   p.k_rows = a.page_size < 64 ? a.page_size : 64;
   p.v_rows = a.page_size < kBN ? a.page_size : kBN;
-  p.sliding_window = a.sliding_window; p.causal = a.stage == G4B_STAGE_CAUSAL; p.o_dtype = a.o.dtype;
+  p.sliding_window = a.sliding_window < (1 << 30) ? a.sliding_window : 1 << 30;    // (no context is longer; sums stay in 32 bits)
+  p.causal = a.stage == G4B_STAGE_CAUSAL; p.o_dtype = a.o.dtype;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = device_status_ptr();
   if (p.status == nullptr) return G4B_ERR_CUDA;

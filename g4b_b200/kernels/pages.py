@@ -15,7 +15,7 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     """``pool[dst_pages[i]] = pool[src_pages[i]]`` in every pool of ``pools``, in one launch
     (``g4b_page_copy``).  ``pools``: torch tensors ``[num_pages, ...]`` of any types, contiguous, with
     one number of pages: the K and V pools of all layers, and the scales of 8-bit ones.
-    ``src_pages, dst_pages [n]`` int32 on the device; negative entries are padding.
+    ``src_pages, dst_pages [n]`` int32 on the device, n at most 65536; negative entries are padding.
 
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status

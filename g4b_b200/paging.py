@@ -191,8 +191,8 @@ class PagedKVManager:
         sequences will write that row.  The new slot gets as many pages of its own behind it as the
         old one has reserved."""
         s = self.slots[slot]
-        if s.filled <= 0:
-            raise ValueError(f"slot {slot} holds no tokens")
+        if not s.active or s.filled <= 0:
+            raise ValueError(f"slot {slot} holds no tokens of a running request")
         free = [i for i in self.free_slots() if i != slot]
         if not free:
             raise RuntimeError("no free slot")

@@ -429,6 +429,9 @@ int g4b_rope_norm_append_packed(const G4bRopePackedArgs* args, void* cuda_stream
  * needs no initial contents and keeps none between calls, but calls that overlap on the GPU (two streams,
  * two captured graphs replayed side by side) each need their own.
  *
+ * Pages that lie wholly in front of a window need not be there any more (sliding_window; their table entries
+ * are not read where no row of the block sees them).
+ *
  * q_starts that decrease or leave [0, N]: nothing is computed, 0x107 in the device status word.  A
  * block-table entry outside the pool reads as zeros and is recorded (0x309), a slot is attended to as
  * far as its table reaches.
@@ -471,7 +474,7 @@ typedef struct G4bPagePool {
 typedef struct G4bPageCopyArgs {
   const G4bPagePool* pools; /* host array of num_pools, read before the call returns */
   int64_t num_pages;
-  G4bTensor src_pages;      /* int32 [n], n <= 2^20 */
+  G4bTensor src_pages;      /* int32 [n], n <= 65536 */
   G4bTensor dst_pages;      /* int32 [n] */
   int32_t num_pools;
   int32_t reserved;

@@ -130,7 +130,7 @@ def test_pages_and_head_dims(cuda, D, page):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,G", [(1, 1), (4, 4), (2, 1), (3, 1), (6, 2), (5, 1), (7, 1), (8, 1), (9, 3), (16, 1), (48, 1), (128, 1), (65, 1)])
+@pytest.mark.parametrize("H,G", [(1, 1), (4, 4), (2, 1), (3, 1), (6, 2), (5, 1), (7, 1), (8, 1), (9, 3), (16, 1), (48, 1), (64, 1), (128, 1), (65, 1)])
 def test_groups(cuda, H, G):
     both(make(H, [150, 3, 270], [150, 70, 300], H=H, G=G, D=128 if H > 16 else 256))
 
@@ -264,6 +264,38 @@ def test_bad_entries_are_recorded_and_bounded(cuda):
     run(c)
     check(c, before, slots=(0,))
     _cabi.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_pages_in_front_of_the_window_may_be_gone(cuda, page):
+    """Their entries are -1 or name somebody else's pages, full of NaN: nothing is recorded, nothing read."""
+    c = make(33, [300, 1, 64], [900, 2000, 1500], page=page, H=4, G=2)
+    window = 200
+    for b, (r, t) in enumerate(zip(c["rows"], c["t"])):
+        first = max(0, t - r - window + 1) // page
+        c["table"][b, :first] = -1
+    before = c["o"].clone()
+    run(c, sliding_window=window)
+    assert _cabi.device_status() == 0
+    c["table"].clamp_(min=0)
+    check(c, before, sliding_window=window)
+
+
+@pytest.mark.gpu
+def test_output_over_the_queries(cuda):
+    c = make(34, [300, 1, 64], [300, 9000, 64], H=8, G=2)
+    d = {**c, "q": c["q"].clone()}
+    c["o"] = c["q"]
+    run(c)
+    d["o"] = c["o"]
+    check(d, d["q"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1])
+def test_windows_longer_than_any_context(cuda, window):
+    both(make(35, [100, 70], [60, 300]), sliding_window=window)
 
 
 @pytest.mark.gpu

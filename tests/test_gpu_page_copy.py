@@ -63,6 +63,8 @@ def test_refusals():
         pages.copy_pages([a], i32([[0]]), i32([[1]]), stream=0)
     with pytest.raises(TypeError):
         pages.copy_pages([a], [0], [1], stream=0)
+    with pytest.raises(ValueError, match="65536"):
+        pages.copy_pages([a], torch.zeros(65537, dtype=torch.int32), torch.zeros(65537, dtype=torch.int32), stream=0)
 
 
 @pytest.mark.launches_allowed

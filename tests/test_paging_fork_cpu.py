@@ -83,6 +83,9 @@ def test_fork_of_a_fork_and_of_nothing():
     m.free(c)
     with pytest.raises(ValueError, match="no tokens"):
         m.fork(c)
+    m.retire(b)
+    with pytest.raises(ValueError, match="no tokens of a running"):
+        m.fork(b)
 
 
 def test_fork_drops_cached_pages_but_not_its_own():
