@@ -1,9 +1,10 @@
 """Packed norm + rotary (several axes) + append against the formulas in 64 bits.
 
 Tolerance.  With u = 2^-24: a normalised element is off by at most 17 u relative (the sum of squares' at most
-20 additions count half in the root, 2 ulp for rsqrtf, three products), sine and cosine by 4 u (2 ulp, and
-a reduced angle rounded to 32 bits: 2^-26 turns), the two products and the sum of the rotation by 3 u: 24 u
-(|a| + |c|) for the pair (a, c); 32 u is allowed.  On top of it half a step of the output type."""
+20 additions count half in the root, 2 ulp for rsqrtf, three products); sine and cosine by 12 u where the outputs have 16 bits
+(2^-21.2 for the fast functions on [-pi, pi], and an angle off by 2^-26 turns, by the rounding of 2 pi and of the
+product), by 4 u where they have 32; the two products and the sum of the rotation by 3 u: 32 u (|a| + |c|) for the
+pair (a, c).  On top of it half a step of the output type."""
 import math
 
 import pytest
