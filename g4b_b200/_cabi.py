@@ -179,6 +179,8 @@ EXPORTS = {
 }
 
 _lib = None
+_fast = None                # the module of csrc/views.cpp
+_address: dict = {}         # entry point -> its address in the loaded library
 
 
 def lib_path() -> Path:
@@ -201,10 +203,56 @@ def load() -> ctypes.CDLL:
             fn.restype = restype
             fn.argtypes = argtypes
         _lib = lib
+        _address.update({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTS})
+        _load_fast()
     return _lib
 
 
+def _load_fast() -> None:
+    """The compiled argument packing, where it has been built and torch is in use; without it the Python code packs."""
+    global _fast
+    path = _LIB_PATH.parent / "_views.so"
+    if _fast is None and "torch" in sys.modules and path.exists():
+        import importlib.util
+
+        spec = importlib.util.spec_from_file_location("_views", path)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError:      # built against another torch
+            return
+        _fast = module
+
+
+def call(name: str, args_type, tensors: tuple, tail: bytes, stream) -> None:
+    """Entry point ``name`` on an argument struct that is the views of ``tensors`` (None: not given) and ``tail``."""
+    lib = _lib if _lib is not None else load()
+    if _fast is not None:
+        rc = _fast.call(_address[name], _validate_only_depth == 0, stream if stream is None or type(stream) is int else current_stream(stream),
+                        tail, tensors)
+        if rc is not None:
+            if rc != 0:
+                check(rc)
+            return
+    a = args_type.from_buffer_copy(views(*tensors) + tail)
+    check(getattr(lib, name)(ctypes.byref(a), current_stream(stream)))
+
+
 _dtype_codes: dict = {}     # dtype objects seen so far: spelling one out costs more than the rest of a view
+
+
+def page_copy(pools: list, src_pages, dst_pages, stream) -> bool:
+    """``g4b_page_copy`` through the compiled packing; False where that is for the Python code (or an error of its)."""
+    if _lib is None:
+        load()
+    if _fast is None:
+        return False
+    rc = _fast.page_copy(_address["g4b_page_copy"], _validate_only_depth == 0,
+                         stream if stream is None or type(stream) is int else current_stream(stream), pools, src_pages, dst_pages)
+    if rc is None:
+        return False
+    check(rc)
+    return True
 
 
 def dtype_code(dt) -> int:
@@ -294,6 +342,10 @@ def _view_bytes(t) -> bytes:
 
 def views(*tensors) -> bytes:
     """The C views of tensor-likes (None: not given) behind one another, as bytes."""
+    if _fast is not None:
+        packed = _fast.views(_validate_only_depth == 0, tensors)
+        if packed is not None:
+            return packed
     torch = sys.modules.get("torch")
     if torch is None:
         return b"".join([_ABSENT if t is None else _view_bytes(t) for t in tensors])

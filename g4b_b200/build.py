@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import hashlib
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -17,6 +18,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 LIB = LIBDIR / "libg4b_attn.so"
+VIEWS = LIBDIR / "_views.so"           # argument packing for torch tensors (a CPython module)
 INCLUDE = PKG.parent / "include"
 
 SOURCES = ["api.cu", "kv_append.cu", "rope_append.cu", "combine.cu", "combine_exchange.cu", "decode.cu", "decode_stream.cu", "decode_static.cu", "tensor_map.cu", "prefill_sm100.cu",
@@ -38,13 +40,41 @@ def _nvcc() -> str:
     return cand
 
 
+def _torch_version() -> str:
+    """Of the torch that views.cpp is built against; "" where there is none (the library needs none)."""
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return ""
+
+
 def _digest() -> str:
     h = hashlib.sha256()
-    for f in sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))):
+    for f in sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.cpp")) + list(INCLUDE.glob("*.h"))):
         h.update(f.name.encode())
         h.update(f.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())
+    h.update(_torch_version().encode())
     return h.hexdigest()
+
+
+def _build_views() -> None:
+    """The CPython module that packs torch tensors (csrc/views.cpp), against the torch that is installed."""
+    if not _torch_version():
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    nvcc_root = Path(_nvcc()).resolve().parents[1]
+    libs = Path(torch.__file__).parent / "lib"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{d}" for d in include_paths()], f"-I{sysconfig.get_paths()['include']}", f"-I{nvcc_root / 'include'}",
+           str(CSRC / "views.cpp"), "-o", str(VIEWS), f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for views.cpp:\n{res.stdout}\n{res.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -54,7 +84,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     objdir.mkdir(exist_ok=True)
     stamp = LIBDIR / "build.stamp"
     digest = _digest()
-    if not force and LIB.exists() and stamp.exists() and stamp.read_text() == digest:
+    if not force and LIB.exists() and (VIEWS.exists() or not _torch_version()) and stamp.exists() and stamp.read_text() == digest:
         return LIB
     nvcc = _nvcc()
     extra = ["-Xptxas", "-v"] if verbose else []
@@ -69,8 +99,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             sys.stderr.write(res.stderr)
         return obj
 
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 1)) as ex:
+        views = ex.submit(_build_views)
         objs = list(ex.map(compile_one, SOURCES))
+        views.result()
     cmd = [nvcc, "-shared", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

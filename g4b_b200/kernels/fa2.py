@@ -214,8 +214,7 @@ def flash_attention_packed(q, k_pool, v_pool, o, q_starts, time_dim_sizes, *, bl
 
     ``workspace``: device memory of at least ``packed_workspace_bytes(N, B, H, G)`` bytes, which a program
     allocates once; calls that may overlap on the GPU need one each.  Returns None."""
-    a = _cabi.G4bPackedAttnArgs.from_buffer_copy(
-        _cabi.views(q, o, k_pool, v_pool, q_starts, time_dim_sizes, block_tables, workspace)
-        + _PACKED_TAIL.pack(page_size, stage, sliding_window or 0, scale))
-    _cabi.check(_cabi.load().g4b_flash_attention_packed(ctypes.byref(a), _cabi.current_stream(stream)))
+    _cabi.call("g4b_flash_attention_packed", _cabi.G4bPackedAttnArgs,
+               (q, o, k_pool, v_pool, q_starts, time_dim_sizes, block_tables, workspace),
+               _PACKED_TAIL.pack(page_size, stage, sliding_window or 0, scale), stream)
     return None

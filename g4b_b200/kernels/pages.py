@@ -20,8 +20,9 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status
     word says so), so what it does never depends on the order of the blocks.  Returns None."""
-    # (the pools are dozens: each thing is asked of all of them at once, the cheapest way)
     pools = list(pools)
+    if _cabi.page_copy(pools, src_pages, dst_pages, stream):
+        return None
     shapes = [p.shape for p in pools]
     num_pages = shapes[0][0] if pools and shapes[0] else 0
     for device in {p.get_device() for p in pools}:

@@ -135,13 +135,15 @@ def rope_norm_append_packed(
     ``pair_axis [D/2]`` (uint8) deals the pairs to time, height and width in sections or in turn.
     The rotated q goes to ``q_out`` (any float dtype) or back into ``q``; k and v go to their slots'
     pages.  No counterpart in the reference."""
-    a = _cabi.G4bRopePackedArgs.from_buffer_copy(
-        _cabi.views(q, k, v, q_out, rope_freqs, positions, pair_axis, q_starts, time_dim_sizes, q_rmsnorm_w, k_rmsnorm_w,
-                    k_pool, v_pool, block_tables)
-        + _PACKED_TAIL.pack(rmsnorm_eps, page_size, 1 if norm_qk else 0, 1 if norm_v else 0))
-    if positions is not None and len(positions.shape) == 1:            # one axis
-        n, step = a.positions.shape[0], a.positions.stride[0]
-        a.positions.ndim, a.positions.shape[0], a.positions.stride[0] = 2, 1, 0
-        a.positions.shape[1], a.positions.stride[1] = n, step
+    tensors = (q, k, v, q_out, rope_freqs, positions, pair_axis, q_starts, time_dim_sizes, q_rmsnorm_w, k_rmsnorm_w, k_pool, v_pool,
+               block_tables)
+    tail = _PACKED_TAIL.pack(rmsnorm_eps, page_size, 1 if norm_qk else 0, 1 if norm_v else 0)
+    if positions is None or len(positions.shape) != 1:
+        _cabi.call("g4b_rope_norm_append_packed", _cabi.G4bRopePackedArgs, tensors, tail, stream)
+        return None
+    a = _cabi.G4bRopePackedArgs.from_buffer_copy(_cabi.views(*tensors) + tail)      # one axis
+    n, step = a.positions.shape[0], a.positions.stride[0]
+    a.positions.ndim, a.positions.shape[0], a.positions.stride[0] = 2, 1, 0
+    a.positions.shape[1], a.positions.stride[1] = n, step
     _cabi.check(_cabi.load().g4b_rope_norm_append_packed(ctypes.byref(a), _cabi.current_stream(stream)))
     return None
