@@ -6,9 +6,10 @@
 // Pure streaming, every byte read once and written once.  A block takes one page pair, a warp of
 // it 4 KB pieces of the pair's run in the pools, eight 16-byte loads a lane in flight before the
 // first store; how many blocks share a pair is chosen so that a fork of a few pages still
-// occupies every SM.  Measured (graph replay): 2100 pages in 16 pools of 16 KB pages 175.4 us = 6280 GB/s read + written,
-// 0.96 of the copy (176.7 without the streaming hints; 175.1 with 16 loads in flight, but then 4 pages in 48 pools
-// take 3.5 us instead of 2.9).
+// occupies every SM.  Measured on three sets of pools in turn: 2100 pages in 16 pools of 16 KB pages 178.2 us = 6180 GB/s
+// read + written, 0.94 of the copy (180.8 with streaming hints on loads and stores, which gain 0.7 % where one set
+// is copied over and over and lose 14 % on 301 pages of 8-bit pools, 8.3 -> 9.5 us; 177.0 with 16 loads in flight,
+// but then 4 pages in 48 pools take 3.5 us instead of 2.9).
 //
 // A pair list can contradict itself (one destination named twice, or a page that is read and
 // written in the same call), and what it would do then depended on which block came first.  Every
@@ -48,12 +49,12 @@ __device__ __forceinline__ void copy_piece(const char* from, char* to, int bytes
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int k = at + i * 32 + lane;
-      if (k < n) x[i] = __ldcs(a + k);
+      if (k < n) x[i] = a[k];
     }
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int k = at + i * 32 + lane;
-      if (k < n) __stcs(b + k, x[i]);
+      if (k < n) b[k] = x[i];
     }
   }
 }

@@ -26,7 +26,13 @@
 //   context ends inside a group the producer zeroes the rest of V itself (it may hold anything, and
 //   0 x NaN would poison the accumulator); K needs no such care, its scores are replaced.
 //
-// Output rows are turned through shared memory so that a warp stores 128-byte row pieces.
+// Output rows are turned through shared memory, so that they leave as TMA boxes or as 128-byte row pieces.
+//
+// Measured (8 / 2 heads, 16-row pages, bf16; 300 to 340 us by box and clock): prompts of 8192, 5000, 2500 and 701 rows at head
+// dim 256, 0.405 TFLOP: 1.2 to 1.35 PFLOP/s, tensor pipe 75 % active; bound by the tensor pipe and the power it draws.  4 x
+// 8192 rows with 64-row pages 741 us = 1484 TFLOP/s.  A window of 512 keys: 68 to 80 us for 0.052 TFLOP, bound by an item's end
+// (6500 cycles for five tiles of 2450).  Head dim 128: 87 to 99 us for 0.067 TFLOP, bound by the softmax warps' latency (2070
+// cycles a tile for 1024 of tensor work).  Three prompts of 62 rows in all: 12 us, of which the list 1.7, the first loads 3.
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 
