@@ -429,6 +429,8 @@ int g4b_rope_norm_append_packed(const G4bRopePackedArgs* args, void* cuda_stream
  * needs no initial contents and keeps none between calls, but calls that overlap on the GPU (two streams,
  * two captured graphs replayed side by side) each need their own.
  *
+ * Rows past a slot's context, pages of nobody and other slots' rows may hold anything.  Inside a slot's own context
+ * V should be finite: a row's weight for a key it does not see is 0, and 0 x NaN is NaN.
  * Pages that lie wholly in front of a window need not be there any more (sliding_window; their table entries
  * are not read where no row of the block sees them).
  *
