@@ -555,8 +555,8 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
   give_registers();       // (all four warps of the group, the idle one too)
   if (warp == 8 || warp == 10) {
     // =============================== producers ===============================
-    // Warp 8 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB, 32 of them a tile, and one
-    // warp does not issue them as fast as the tensor pipe consumes them (4 prompts of 8192 rows, 8 / 2 heads,
+    // Warp 8 fetches Q and K, warp 10 V: a page of 16 rows is a box of 2 KB (V: 4), two dozen of them a tile, and one
+    // warp does not issue them as fast as the tensor pipe consumes them (with 2 KB boxes of V too: 4 prompts of 8192 rows, 8 / 2 heads,
     // pages of 16: 1153 us with one producer warp, 846 us with two).
     // Each has its own half of the ring: with one ring the V warp, which nothing holds up at an item switch, came to a
     // slot whose use before (a K chunk) was not even issued, and the slot's one-bit phase cannot tell that apart.
@@ -605,8 +605,9 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       const int st_base = for_v ? kSt : 0;
       auto wait_empty = [&](int st) { return wait_lane0(ptx::smem_u32(&bars->kv_empty[st]), ((cc / kSt) & 1) ^ 1, kErrKvEmpty); };
       // K chunk = this CTA's 64 keys of the tile x kD (slabs of [64 rows x 64 d]); V chunk = all 128 keys x
-      // this CTA's half of the head dim (slabs of [128 rows x 64 d]).  Lane i fetches the i-th group of
-      // rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
+      // this CTA's half of the head dim, group by group of rows (a group: slabs of [v_rows x 64 d]), since a step of
+      // the product takes 16 keys and does not care where the next 16 lie: one box a group, where K needs one a group and
+      // slab (sixteen prompts over pages of 16: 52.8 -> 51.2 us).  Lane i fetches the i-th group of rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
       auto load_k = [&](int j) {
         const int key0 = (it.tile_lo + j) * kBN + 64 * (int)rank + lane * p.k_rows;
         const int boxes = 64 / p.k_rows;
@@ -643,13 +644,10 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         __syncwarp();
         uint8_t* chunk = sRing + st * kChunk;
         if (lane < boxes) {
-          const uint32_t dst = ptx::smem_u32(chunk + lane * p.v_rows * 128);
-#pragma unroll
-          for (int s = 0; s < kSlabs / 2; ++s) {
-            const int d = (int)rank * kHalfCols + s * 64;
-            if (dirty != 0) ptx::tma_load_4d_hint(dst + s * 16384, &v_map, bar, d, key0 & page_mask, g, page, pol_kv);
-            else ptx::tma_load_4d_pair(dst + s * 16384, &v_map, bar, d, key0 & page_mask, g, page, pol_kv);
-          }
+          const uint32_t dst = ptx::smem_u32(chunk + lane * p.v_rows * (128 * kSlabs / 2));
+          const int slab = (int)rank * (kSlabs / 2);
+          if (dirty != 0) ptx::tma_load_5d_hint(dst, &v_map, bar, 0, key0 & page_mask, slab, g, page, pol_kv);
+          else ptx::tma_load_5d_pair(dst, &v_map, bar, 0, key0 & page_mask, slab, g, page, pol_kv);
         }
         __syncwarp();
         if (dirty != 0) {
@@ -659,7 +657,8 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
           const int rows = p.v_rows - dirty;
           for (int i = lane; i < rows * 8 * (kSlabs / 2); i += 32) {
             const int s = i / (rows * 8), at = i - s * rows * 8;
-            *reinterpret_cast<uint4*>(chunk + s * 16384 + live * 128 + at * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(chunk + (live - dirty) * (128 * kSlabs / 2) + s * p.v_rows * 128 + dirty * 128 + at * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
@@ -683,7 +682,12 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       constexpr uint32_t idesc_pv = ptx::make_idesc_f16(PackT<T>::kFmt, 256, kD, 0, 1);
       constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // SBO 1024 B, version 1, SWIZZLE_128B
       constexpr uint32_t kLoKMajor = 1u << 16;
-      constexpr uint32_t kLoVMajor = (16384u >> 4) << 16;   // LBO: 64-wide slabs of 128 rows are 16 KB apart
+      const uint32_t v_slab = (uint32_t)p.v_rows * 128;       // LBO: 64-wide slabs of a group of rows lie behind one another
+      const uint32_t lo_v_major = (v_slab >> 4) << 16;
+      uint32_t v_step[8];                                     // where the 16 keys of a step lie (one slab: behind one another)
+#pragma unroll
+      for (int k16 = 0; k16 < 8; ++k16)
+        v_step[k16] = (k16 * 16 / p.v_rows * p.v_rows * (128 * kSlabs / 2) + k16 * 16 % p.v_rows * 128) >> 4;
       const uint32_t q_lo = (ptx::smem_u32(sQ) >> 4) | kLoKMajor;
       const uint32_t ring_lo = ptx::smem_u32(sRing) >> 4;
       auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity)); };
@@ -736,7 +740,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             ok = false; return;
           }
           const int t = tg + j;
-          const uint32_t v_lo = (ring_lo + st * (kChunk >> 4)) | kLoVMajor;
+          const uint32_t v_lo = (ring_lo + st * (kChunk >> 4)) | lo_v_major;
           const uint32_t p_tmem = tmem + ((t & 1) ? kColS1 : kColS0);
           if (j == 0 && n_done > 0) {
             // the first product of an item overwrites O: the previous item's O must have been read
@@ -758,7 +762,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
               for (int i = 0; i < 4; ++i) {
                 // part 0: keys 0..31 and 64..95 (k16 = 0,1,4,5); part 1: the rest
                 const int k16 = (i >> 1) * 4 + part * 2 + (i & 1);
-                const uint64_t vdesc = ptx::desc64(v_lo + (k16 * 2048 >> 4), kDescHi);
+                const uint64_t vdesc = ptx::desc64(v_lo + (kSlabs == 2 ? k16 * 2048 >> 4 : v_step[k16]), kDescHi);
                 ptx::mma_ts_pair(tmem + kColO, p_tmem + k16 * 8, vdesc, idesc_pv, (j | part | i) != 0);
                 if (precise) ptx::mma_ts_pair(tmem + kColO, p_tmem + 64 + k16 * 8, vdesc, idesc_pv, 1u);
               }
@@ -1345,9 +1349,13 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
     const uint64_t P = (uint64_t)a.page_size;
     const uint64_t pdims[4] = {(uint64_t)D, P, (uint64_t)G, (uint64_t)p.num_pages};
     const uint64_t pstr[3] = {(uint64_t)D * esz, P * D * esz, (uint64_t)G * P * D * esz};
-    const uint32_t kbox[4] = {64, (uint32_t)p.k_rows, 1, 1}, vbox[4] = {64, (uint32_t)p.v_rows, 1, 1};
+    const uint32_t kbox[4] = {64, (uint32_t)p.k_rows, 1, 1};
+    // V with the head dim as slabs of 64: a box is the rows of a group and a CTA's slabs
+    const uint64_t vdims[5] = {64, P, (uint64_t)D / 64, (uint64_t)G, (uint64_t)p.num_pages};
+    const uint64_t vstr[4] = {(uint64_t)D * esz, 128, P * D * esz, (uint64_t)G * P * D * esz};
+    const uint32_t vbox[5] = {64, (uint32_t)p.v_rows, (uint32_t)(D / 128), 1, 1};
     if ((rc = encode_map(&km, a.k_pool.dtype, 4, a.k_pool.ptr, pdims, pstr, kbox, "k_pool"))) return rc;
-    if ((rc = encode_map(&vm, a.v_pool.dtype, 4, a.v_pool.ptr, pdims, pstr, vbox, "v_pool"))) return rc;
+    if ((rc = encode_map(&vm, a.v_pool.dtype, 5, a.v_pool.ptr, vdims, vstr, vbox, "v_pool"))) return rc;
   }
   // The output as boxes of the 32 rows that a warp holds: 32 / (heads of a group) tokens, or 32 heads of one.  Other
   // group sizes, f32, and layouts that a descriptor cannot express (the driver refuses it) are stored by the warps.
