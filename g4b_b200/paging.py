@@ -87,6 +87,8 @@ class _Slot:
     pages: list[int] = field(default_factory=list)   # page ids in sequence order
     tokens: list[int] = field(default_factory=list)  # tokens whose K/V those pages hold (or will, once prefilled)
     filled: int = 0                                  # leading tokens whose K/V a launched step has written
+    length: int = 0                                  # tokens the sequence surely holds (a padded chunk's padding is not counted)
+    reach: int = 0                                   # ... and may hold: rows from `length` on are padding as far as is known here
     active: bool = False
     retired_at: int = -1                             # tick of retirement, for eviction order
 
@@ -150,7 +152,7 @@ class PagedKVManager:
                 s.pages = list(self.slots[donor].pages[:n_pages])
                 self.alloc.retain(s.pages)
         s.tokens = list(tokens)
-        s.filled = n
+        s.filled = s.length = s.reach = n
         s.active = True
         s.retired_at = -1
         self._write_row(slot)
@@ -174,7 +176,7 @@ class PagedKVManager:
         behind as a prefix cache (``retire``).  Pages that other slots share stay theirs."""
         s = self.slots[slot]
         self.alloc.release(s.pages)
-        s.pages, s.tokens, s.filled = [], [], 0
+        s.pages, s.tokens, s.filled, s.length, s.reach = [], [], 0, 0, 0
         s.active, s.retired_at = False, -1
         self.cache_offsets[slot] = self.time_dim_sizes[slot] = 0
         self.user_phase[slot] = PHASE_UNALLOCATED
@@ -188,10 +190,12 @@ class PagedKVManager:
 
         Full pages are shared.  The page of the slot's last token is copied: the state may already
         have been advanced to a token that only the next step writes (``advance_decode``), and both
-        sequences will write that row.  The new slot gets as many pages of its own behind it as the
-        old one has reserved."""
+        sequences will write that row.  Behind a padded prefill the last token is the prompt's
+        (``place_request``), whose padding both sequences will write over; pages that hold
+        nothing else are copied too, since a caller may have gone on past that prompt.  The new
+        slot gets as many pages of its own behind it as the old one has reserved."""
         s = self.slots[slot]
-        if not s.active or s.filled <= 0:
+        if not s.active or s.length <= 0:
             raise ValueError(f"slot {slot} holds no tokens of a running request")
         free = [i for i in self.free_slots() if i != slot]
         if not free:
@@ -199,19 +203,20 @@ class PagedKVManager:
         new = min(free, key=lambda i: len(self.slots[i].pages))
         t = self.slots[new]
         self.alloc.release(t.pages)
-        t.pages, t.tokens, t.filled, t.retired_at = [], [], 0, -1
+        t.pages, t.tokens, t.filled, t.length, t.reach, t.retired_at = [], [], 0, 0, 0, -1
         self._write_row(new)
-        shared = (s.filled - 1) // self.page_size
+        shared, last = (s.length - 1) // self.page_size, (s.reach - 1) // self.page_size
         need = len(s.pages) - shared
         self._make_room(need, keep=slot)
         own = self.alloc.alloc(need)
         self.alloc.retain(s.pages[:shared])
         t.pages = list(s.pages[:shared]) + own
-        t.tokens, t.filled, t.active = list(s.tokens), s.filled, True
+        t.tokens, t.filled, t.active = list(s.tokens), min(s.filled, s.reach), True
+        t.length, t.reach = s.length, s.reach
         self.cache_offsets[new], self.time_dim_sizes[new] = self.cache_offsets[slot], self.time_dim_sizes[slot]
         self.user_phase[new] = self.user_phase[slot]
         self._write_row(new)
-        return new, [(s.pages[shared], own[0])]
+        return new, list(zip(s.pages[shared:last + 1], own))
 
     def compact(self) -> tuple[np.ndarray, np.ndarray]:
         """Moves every page in use to the front of the pool, so that the pages behind
@@ -256,7 +261,7 @@ class PagedKVManager:
         for i in retired:
             s = self.slots[i]
             self.alloc.release(s.pages)
-            s.pages, s.tokens, s.filled = [], [], 0
+            s.pages, s.tokens, s.filled, s.length, s.reach = [], [], 0, 0, 0
             self._write_row(i)
             if self.alloc.free_pages >= need:
                 return
@@ -276,7 +281,7 @@ class PagedKVManager:
         iff ``time_sizes_after[b] > 0`` (the scheduler passes zeros for idle slots,
         g4b/scheduler.py:141-147); its table is grown to ``time_sizes_after[b]`` tokens, which
         counts the whole padded chunk (g4b/scheduler.py:166-172)."""
-        return self._prepare(cache_offsets, time_sizes_after, PHASE_PREFILL, reserve=0)
+        return self._prepare(cache_offsets, time_sizes_after, PHASE_PREFILL, reserve=0, padded=True)
 
     def prepare_decode_inputs(self, token_cols, cache_offsets, time_sizes_after, sample_positions=None):
         """Same arguments as ``Model.prepare_decode_inputs``.  The reference uploads decode state
@@ -284,7 +289,7 @@ class PagedKVManager:
         ahead: ``decode_reserve_pages`` beyond the one the next token falls in."""
         return self._prepare(cache_offsets, time_sizes_after, PHASE_DECODE, reserve=self.decode_reserve_pages)
 
-    def _prepare(self, cache_offsets, time_sizes_after, phase, reserve):
+    def _prepare(self, cache_offsets, time_sizes_after, phase, reserve, padded=False):
         for b in range(self.max_batch):
             live = time_sizes_after[b] > 0
             self.cache_offsets[b] = cache_offsets[b]
@@ -295,6 +300,9 @@ class PagedKVManager:
                 self.ensure(b, max(want, int(time_sizes_after[b])))
                 s = self.slots[b]
                 s.filled = max(s.filled, int(time_sizes_after[b]))
+                s.length = s.reach = int(time_sizes_after[b])
+                if padded:         # the prompt may end inside the chunk; its first token is one in any case
+                    s.length = min(s.reach, max(len(s.tokens), int(cache_offsets[b]) + 1))
         return self.block_tables, self.cache_offsets, self.time_dim_sizes, self.user_phase
 
     def prepare_packed_inputs(self, row_counts, time_sizes_after):
@@ -327,7 +335,9 @@ class PagedKVManager:
                 continue
             self.cache_offsets[b] += 1
             self.time_dim_sizes[b] += 1
-            self.slots[b].filled = max(self.slots[b].filled, int(self.time_dim_sizes[b]))
+            s = self.slots[b]
+            s.length = s.reach = int(self.time_dim_sizes[b])
+            s.filled = max(s.filled, s.length)
             if self.decode_steps_covered(b) < 0:
                 raise RuntimeError(f"slot {b} ran past its reserved pages")
             if self.decode_steps_covered(b) == 0 and int(self.time_dim_sizes[b]) < self.max_pages * self.page_size:
