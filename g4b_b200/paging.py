@@ -193,7 +193,8 @@ class PagedKVManager:
         sequences will write that row.  Behind a padded prefill the last token is the prompt's
         (``place_request``), whose padding both sequences will write over; pages that hold
         nothing else are copied too, since a caller may have gone on past that prompt.  The new
-        slot gets as many pages of its own behind it as the old one has reserved."""
+        slot gets as many pages of its own behind it as the old one has reserved, and the old one's
+        state; where the old one sat out the last step, a state of all its tokens, in no phase."""
         s = self.slots[slot]
         if not s.active or s.length <= 0:
             raise ValueError(f"slot {slot} holds no tokens of a running request")
@@ -213,8 +214,12 @@ class PagedKVManager:
         t.pages = list(s.pages[:shared]) + own
         t.tokens, t.filled, t.active = list(s.tokens), min(s.filled, s.reach), True
         t.length, t.reach = s.length, s.reach
-        self.cache_offsets[new], self.time_dim_sizes[new] = self.cache_offsets[slot], self.time_dim_sizes[slot]
-        self.user_phase[new] = self.user_phase[slot]
+        if self.user_phase[slot] != PHASE_UNALLOCATED and self.time_dim_sizes[slot] == s.reach:
+            self.cache_offsets[new], self.time_dim_sizes[new] = self.cache_offsets[slot], self.time_dim_sizes[slot]
+            self.user_phase[new] = self.user_phase[slot]
+        else:
+            self.cache_offsets[new] = self.time_dim_sizes[new] = s.length
+            self.user_phase[new] = PHASE_UNALLOCATED
         self._write_row(new)
         return new, list(zip(s.pages[shared:last + 1], own))
 

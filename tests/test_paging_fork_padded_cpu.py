@@ -1,9 +1,9 @@
-"""Forks of slots whose last prefill chunk was padded: no page that either sequence still
+"""Forks of slots whose last prefill chunk was padded, or that sat out the last step: no page that either sequence still
 writes is shared, and every row that holds a token is in both."""
 import numpy as np
 import pytest
 
-from g4b_b200.paging import PHASE_DECODE, PagedKVManager
+from g4b_b200.paging import PHASE_DECODE, PHASE_UNALLOCATED, PagedKVManager
 
 PAGE = 16
 
@@ -83,3 +83,33 @@ def test_a_chunk_past_the_prompt_counts_from_its_first_token():
     pa, pb = m.slots[a].pages, m.slots[b].pages
     assert pa[0] == pb[0] or (pa[0], pb[0]) in copies
     assert copies == list(zip(pa[1:4], pb[1:4]))
+
+
+def test_a_slot_that_sat_out_the_last_step_forks_with_all_its_tokens():
+    m = manager()
+    a = prefill(m, 40, 40)
+    other, _ = m.place_request(list(range(1000, 1010)))
+    rows, after = [0] * 4, [0] * 4
+    rows[other] = after[other] = 10
+    m.prepare_packed_inputs(rows, after)
+    b, copies = m.fork(a)
+    assert copies == [(m.slots[a].pages[2], m.slots[b].pages[2])]
+    assert m.time_dim_sizes[b] == 40 and m.cache_offsets[b] == 40 and m.user_phase[b] == PHASE_UNALLOCATED
+    rows, after = [0] * 4, [0] * 4
+    for s in (a, b):
+        rows[s], after[s] = 1, 41
+    m.prepare_packed_inputs(rows, after)
+    assert all(m.alloc.refcount(m.slots[s].pages[2]) == 1 for s in (a, b))
+
+
+def test_a_prefix_that_was_just_placed_forks_at_its_own_length():
+    """Nothing of the state that the slot's last request left behind is taken over."""
+    m = manager(prefill_chunk=16)
+    a = prefill(m, 70, 16)
+    decode_at(m, [71 if b == a else 0 for b in range(4)])
+    m.retire(a)
+    slot, pos = m.place_request(list(range(40)) + [7, 8, 9])
+    assert slot == a and pos == 32
+    b, copies = m.fork(slot)
+    assert m.time_dim_sizes[b] == 32 and m.user_phase[b] == PHASE_UNALLOCATED
+    assert copies == [(m.slots[a].pages[1], m.slots[b].pages[1])]
