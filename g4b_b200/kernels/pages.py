@@ -19,7 +19,8 @@ def copy_pages(pools, src_pages, dst_pages, *, stream=None):
 
     A page may be copied to many others.  A list that names one destination twice, or reads a
     page that it also writes, is not followed there (the entry is skipped and the device status
-    word says so), so what it does never depends on the order of the blocks.  Returns None."""
+    word says so), so what it does never depends on the order of the blocks; lists handed out by several
+    calls of the manager go through ``g4b_b200.paging.copy_stages`` first.  Returns None."""
     pools = list(pools)
     if _cabi.page_copy(pools, src_pages, dst_pages, stream):
         return None

@@ -35,6 +35,32 @@ def shared_prefix_length(a, b) -> int:
     return n
 
 
+def copy_stages(copies) -> list[tuple[np.ndarray, np.ndarray]]:
+    """The ``(src, dst)`` pairs of several ``PagedKVManager.fork`` calls, and of a ``compact``, in the order they were
+    handed out and none of them launched yet, as lists for ``kernels.pages.copy_pages`` (int32 arrays), one launch
+    a list, in this order.
+
+    Pages change hands between such calls: a fork may copy a page that the last one only just made, or into one that
+    a freed slot gave back and an earlier copy still reads.  ``copy_pages`` reads a whole list before it writes, and
+    skips entries that contradict one another.  Here a copy of a copy is taken from the first
+    one's source, and a copy into a page that an earlier one reads or writes begins a new list; forks of different
+    sequences are one list."""
+    stages, origin, read = [], {}, set()           # origin: destination -> source, of the list at hand
+    for src, dst in copies:
+        src, dst = int(src), int(dst)
+        if src < 0 or dst < 0 or src == dst:
+            continue
+        if dst in origin or dst in read:
+            stages.append(origin)
+            origin, read = {}, set()
+        src = origin.get(src, src)
+        origin[dst] = src
+        read.add(src)
+    if origin:
+        stages.append(origin)
+    return [(np.fromiter(s.values(), np.int32, len(s)), np.fromiter(s.keys(), np.int32, len(s))) for s in stages]
+
+
 class PageAllocator:
     """Free list + reference counts over ``num_pages`` page ids."""
 
@@ -186,7 +212,9 @@ class PagedKVManager:
         """A second sequence that continues where ``slot`` stands, in a free slot: several samples of
         one prompt, or a beam.  Returns ``(new_slot, copies)``; the caller copies page ``src`` to
         page ``dst`` for every ``(src, dst)`` of ``copies`` on the device
-        (``kernels.pages.copy_pages``), behind the steps launched so far and before the next.
+        (``kernels.pages.copy_pages``), behind the steps launched so far and before the next.  The
+        lists of several calls are launched in the order of the calls, each by itself or all of them
+        through ``copy_stages``, never strung together: one may read what another writes.
 
         Full pages are shared.  The page of the slot's last token is copied: the state may already
         have been advanced to a token that only the next step writes (``advance_decode``), and both
@@ -227,8 +255,8 @@ class PagedKVManager:
         """Moves every page in use to the front of the pool, so that the pages behind
         ``num_pages - free_pages`` hold nothing (a pool can then be shrunk, or its tail lent out).
         Returns ``(src, dst)`` int32 page ids for ``kernels.pages.copy_pages``, to run behind the steps
-        launched so far and before the next, whose block tables are the new ones (``upload``).  No
-        page is both read and written."""
+        launched so far and before the next, whose block tables are the new ones (``upload``), and
+        behind the copies of earlier forks (``copy_stages``).  No page is both read and written."""
         live = np.flatnonzero(self.alloc._refs > 0)
         src = live[live >= len(live)].astype(np.int32)
         holes = np.flatnonzero(self.alloc._refs[: len(live)] == 0)
