@@ -231,11 +231,12 @@ class PagedKVManager:
             raise RuntimeError("no free slot")
         new = min(free, key=lambda i: len(self.slots[i].pages))
         t = self.slots[new]
+        shared, last = (s.length - 1) // self.page_size, (s.reach - 1) // self.page_size
+        need = len(s.pages) - shared
+        self._check_room(need, keep=slot)          # (before anything cached is dropped)
         self.alloc.release(t.pages)
         t.pages, t.tokens, t.filled, t.length, t.reach, t.retired_at = [], [], 0, 0, 0, -1
         self._write_row(new)
-        shared, last = (s.length - 1) // self.page_size, (s.reach - 1) // self.page_size
-        need = len(s.pages) - shared
         self._make_room(need, keep=slot)
         own = self.alloc.alloc(need)
         self.alloc.retain(s.pages[:shared])
@@ -284,6 +285,15 @@ class PagedKVManager:
         s.pages += self.alloc.alloc(need)
         self._write_row(slot)
         return True
+
+    def _check_room(self, need: int, keep: int) -> None:
+        """Raises OutOfPages where ``_make_room`` would, with the cached pages as they are."""
+        refs = self.alloc._refs.copy()
+        for i, s in enumerate(self.slots):
+            if not s.active and i != keep:
+                refs[s.pages] -= 1
+        if int((refs == 0).sum()) < need:
+            raise OutOfPages(f"need {need} pages, {int((refs == 0).sum())} free without the prefix cache")
 
     def _make_room(self, need: int, keep: int) -> None:
         """Drops cached pages of retired slots, oldest first, until ``need`` pages are free."""

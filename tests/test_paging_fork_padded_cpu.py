@@ -3,7 +3,7 @@ writes is shared, and every row that holds a token is in both."""
 import numpy as np
 import pytest
 
-from g4b_b200.paging import PHASE_DECODE, PHASE_UNALLOCATED, PagedKVManager
+from g4b_b200.paging import PHASE_DECODE, PHASE_UNALLOCATED, OutOfPages, PagedKVManager
 
 PAGE = 16
 
@@ -113,3 +113,22 @@ def test_a_prefix_that_was_just_placed_forks_at_its_own_length():
     b, copies = m.fork(slot)
     assert m.time_dim_sizes[b] == 32 and m.user_phase[b] == PHASE_UNALLOCATED
     assert copies == [(m.slots[a].pages[1], m.slots[b].pages[1])]
+
+
+def test_a_fork_that_finds_no_pages_leaves_the_prefix_cache():
+    m = manager(num_pages=9, max_batch=3)
+    old = prefill(m, 32, 16)                              # two pages, cached behind the request
+    m.retire(old)
+    m.prepare_packed_inputs([0] * 3, [0] * 3)
+    a, _ = m.place_request(list(range(500, 510)))
+    m.prepare_packed_inputs([10 if b == a else 0 for b in range(3)], [10 if b == a else 0 for b in range(3)])
+    m.ensure(a, 7 * PAGE)                                 # seven pages reserved, none of them full
+    b, _ = m.place_request([9] * 3)
+    free = m.alloc.free_pages
+    tables = m.block_tables.copy()
+    with pytest.raises(OutOfPages):
+        m.fork(a)
+    assert len(m.slots[old].pages) == 2 and m.alloc.free_pages == free
+    assert (m.block_tables == tables).all()
+    slot, pos = (m.retire(b), m.place_request(list(range(32))))[1]
+    assert pos == 31 // 16 * 16
