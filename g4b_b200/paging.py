@@ -333,14 +333,16 @@ class PagedKVManager:
         return self._prepare(cache_offsets, time_sizes_after, PHASE_DECODE, reserve=self.decode_reserve_pages)
 
     def _prepare(self, cache_offsets, time_sizes_after, phase, reserve, padded=False):
+        for b in range(self.max_batch):            # all pages first: a call that finds none has announced no step
+            if time_sizes_after[b] > 0:
+                want = min(int(time_sizes_after[b]) + reserve * self.page_size, self.max_pages * self.page_size)
+                self.ensure(b, max(want, int(time_sizes_after[b])))
         for b in range(self.max_batch):
             live = time_sizes_after[b] > 0
             self.cache_offsets[b] = cache_offsets[b]
             self.time_dim_sizes[b] = time_sizes_after[b]
             self.user_phase[b] = phase if live else PHASE_UNALLOCATED
             if live:
-                want = min(int(time_sizes_after[b]) + reserve * self.page_size, self.max_pages * self.page_size)
-                self.ensure(b, max(want, int(time_sizes_after[b])))
                 s = self.slots[b]
                 s.filled = max(s.filled, int(time_sizes_after[b]))
                 s.length = s.reach = int(time_sizes_after[b])
