@@ -139,6 +139,7 @@ class PagedKVManager:
         self.user_phase = np.zeros(self.max_batch, dtype=np.uint8)
         self.q_starts = np.zeros(self.max_batch + 1, dtype=np.int32)   # packed steps: slot b owns rows [q_starts[b], q_starts[b+1])
         self.tables_dirty = True
+        self._starts_dirty = True
         self._tick = 0
         self._device = None
 
@@ -364,6 +365,7 @@ class PagedKVManager:
                 raise ValueError(f"slot {b}: {n} new rows of {t} tokens")
         self._prepare([t - n for n, t in zip(rows, after)], after, PHASE_PREFILL, reserve=0)
         self.q_starts[1:] = np.cumsum(rows)
+        self._starts_dirty = True
         return self.q_starts, self.block_tables, self.time_dim_sizes
 
     def decode_steps_covered(self, slot: int) -> int:
@@ -407,12 +409,13 @@ class PagedKVManager:
         }
         self._staging = {k: (torch.empty_like(v).pin_memory() if pin else torch.empty_like(v)) for k, v in self._host.items()}
         self.device_tensors = {k: torch.empty_like(v, device=self._device) for k, v in self._host.items()}
+        self._starts_dirty = True
         self._copied = torch.cuda.Event() if pin else None
         self._copy_pending = False
 
     def upload(self, tables_only_if_dirty: bool = True) -> dict:
         """Copies the host state to the device tensors (asynchronously, on torch's current
-        stream).  The block tables go only when they changed."""
+        stream).  The block tables go only when they changed, the packed rows' starts only behind a new packed step."""
         if self._device is None:
             raise RuntimeError("bind_device() first")
         if self._copy_pending:
@@ -421,9 +424,11 @@ class PagedKVManager:
         for name in ("cache_offsets", "time_dim_sizes", "user_phase", "q_starts", "block_tables"):
             if name == "block_tables" and tables_only_if_dirty and not self.tables_dirty:
                 continue
+            if name == "q_starts" and not self._starts_dirty:
+                continue
             self._staging[name].copy_(self._host[name])
             self.device_tensors[name].copy_(self._staging[name], non_blocking=True)
-        self.tables_dirty = False
+        self.tables_dirty = self._starts_dirty = False
         if self._copied is not None:
             self._copied.record()
             self._copy_pending = True
