@@ -132,19 +132,20 @@ __device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepc
 // the list of items
 // ---------------------------------------------------------------------------------------
 struct SlotRows {
-  int first, n, time;     // rows of q, tokens of the slot (bounded by its table)
+  int first, n, time;     // rows of q, tokens of the slot
+  int keys;               // of those tokens, the ones that its table reaches
   bool bad;
 };
 __device__ __forceinline__ SlotRows slot_rows(const PackedParams& p, int b) {
-  SlotRows s{0, 0, 0, false};
+  SlotRows s{0, 0, 0, 0, false};
   if (b >= p.B) return s;
   const int lo = p.q_starts[b * p.starts_s], hi = p.q_starts[(int64_t)(b + 1) * p.starts_s];
   s.bad = lo < 0 || hi < lo || hi > p.N;
   if (s.bad) return s;
   s.first = lo;
   s.n = hi - lo;
-  const int64_t most = min((int64_t)p.max_pages << p.page_shift, (int64_t)0x7fffff00);
-  s.time = (int)min((int64_t)max(p.times[b * p.time_s], 0), most);
+  s.time = min(max(p.times[b * p.time_s], 0), 0x7fffff00);
+  s.keys = (int)min((int64_t)s.time, (int64_t)p.max_pages << p.page_shift);
   return s;
 }
 
@@ -162,7 +163,7 @@ __device__ __forceinline__ PackedItem block_of(const PackedParams& p, const Slot
   it.row0 = s.first + tok0;
   it.n_tok = min(block, s.n - tok0);
   it.qpos0 = s.time - s.n + tok0;
-  it.window = s.time;
+  it.window = s.keys;
   tiles_of(p, it.qpos0, it.n_tok, it.window, it.tile_lo, it.n_tiles);
   it.slot = slot;
   it.g_part = 0;
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ Packe
     bad |= s.bad;
     const int n = (s.n + block - 1) / block;
     if (n > 0) {
-      const int last = min(s.time, cap), first = p.causal ? min(max(s.time - s.n + block, 0), last) : last;
+      const int last = min(s.keys, cap), first = p.causal ? min(max(s.time - s.n + block, 0), last) : last;
       longest = max(longest, (last + kBN - 1) / kBN);
       cost += (float)n * ((float)(first + last) / (2 * kBN) + 0.5f + kEntryCost);
     }

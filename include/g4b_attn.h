@@ -437,7 +437,7 @@ int g4b_rope_norm_append_packed(const G4bRopePackedArgs* args, void* cuda_stream
  *
  * q_starts that decrease or leave [0, N]: nothing is computed, 0x107 in the device status word.  A
  * block-table entry outside the pool reads as zeros and is recorded (0x309), a slot is attended to as
- * far as its table reaches.
+ * far as its table reaches (its rows keep their positions).
  */
 typedef struct G4bPackedAttnArgs {
   G4bTensor q, o;           /* [N, H, D] views, last stride 1, other strides positive multiples of 16 bytes */
