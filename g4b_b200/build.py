@@ -54,14 +54,27 @@ def _digest() -> str:
         h.update(f.name.encode())
         h.update(f.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())
-    h.update(_torch_version().encode())
+    h.update(f"{_torch_version()} {sys.version}".encode())
     return h.hexdigest()
 
 
-def _build_views() -> None:
-    """The CPython module that packs torch tensors (csrc/views.cpp), against the torch that is installed."""
+def _build_views() -> bool:
+    """The CPython module that packs torch tensors (csrc/views.cpp), against the torch that is installed; False where
+    that cannot be built (no g++, no Python headers, a torch without CUDA).  The library needs none of it: without the
+    module the Python code of _cabi.py packs."""
     if not _torch_version():
-        return
+        VIEWS.unlink(missing_ok=True)
+        return False
+    try:
+        _compile_views()
+    except Exception as e:      # whatever keeps it from being built, the library does not depend on it
+        VIEWS.unlink(missing_ok=True)      # (not one of another torch)
+        sys.stderr.write(f"g4b_b200: argument packing stays in Python, {VIEWS.name} was not built: {e}\n")
+        return False
+    return True
+
+
+def _compile_views() -> None:
     import sysconfig
 
     import torch
@@ -84,7 +97,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     objdir.mkdir(exist_ok=True)
     stamp = LIBDIR / "build.stamp"
     digest = _digest()
-    if not force and LIB.exists() and (VIEWS.exists() or not _torch_version()) and stamp.exists() and stamp.read_text() == digest:
+    # (a module that could not be built is not tried again until something changes)
+    if not force and LIB.exists() and stamp.exists() and stamp.read_text() == digest + (" views" if VIEWS.exists() else ""):
         return LIB
     nvcc = _nvcc()
     extra = ["-Xptxas", "-v"] if verbose else []
@@ -102,12 +116,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 1)) as ex:
         views = ex.submit(_build_views)
         objs = list(ex.map(compile_one, SOURCES))
-        views.result()
+        views_built = views.result()
     cmd = [nvcc, "-shared", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-    stamp.write_text(digest)
+    stamp.write_text(digest + (" views" if views_built else ""))
     return LIB
 
 
