@@ -180,6 +180,7 @@ EXPORTS = {
 
 _lib = None
 _fast = None                # the module of csrc/views.cpp
+_fast_looked_for = False
 _address: dict = {}         # entry point -> its address in the loaded library
 
 
@@ -209,24 +210,33 @@ def load() -> ctypes.CDLL:
 
 
 def _load_fast() -> None:
-    """The compiled argument packing, where it has been built and torch is in use; without it the Python code packs."""
-    global _fast
+    """The compiled argument packing, where it has been built for the torch and the Python that run and torch is in use
+    (whether that was imported before the library was loaded or after); without it the Python code packs."""
+    global _fast, _fast_looked_for
+    torch = sys.modules.get("torch")
+    if _fast_looked_for or not hasattr(torch, "__version__") or not hasattr(torch, "Tensor"):     # (not there, or being imported)
+        return
+    _fast_looked_for = True
     path = _LIB_PATH.parent / "_views.so"
-    if _fast is None and "torch" in sys.modules and path.exists():
-        import importlib.util
+    if not path.exists():
+        return
+    import importlib.util
 
-        spec = importlib.util.spec_from_file_location("_views", path)
-        try:
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-        except ImportError:      # built against another torch
-            return
+    spec = importlib.util.spec_from_file_location("_views", path)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError:          # symbols that this torch does not have
+        return
+    if getattr(module, "built_for", None) == f"{torch.__version__} {sys.version.split()[0]} {sys.implementation.cache_tag}":
         _fast = module
 
 
 def call(name: str, args_type, tensors: tuple, tail: bytes, stream) -> None:
     """Entry point ``name`` on an argument struct that is the views of ``tensors`` (None: not given) and ``tail``."""
     lib = _lib if _lib is not None else load()
+    if not _fast_looked_for:
+        _load_fast()
     if _fast is not None:
         rc = _fast.call(_address[name], _validate_only_depth == 0, stream if stream is None or type(stream) is int else current_stream(stream),
                         tail, tensors)
@@ -245,6 +255,8 @@ def page_copy(pools: list, src_pages, dst_pages, stream) -> bool:
     """``g4b_page_copy`` through the compiled packing; False where that is for the Python code (or an error of its)."""
     if _lib is None:
         load()
+    if not _fast_looked_for:
+        _load_fast()
     if _fast is None:
         return False
     rc = _fast.page_copy(_address["g4b_page_copy"], _validate_only_depth == 0,
@@ -342,6 +354,8 @@ def _view_bytes(t) -> bytes:
 
 def views(*tensors) -> bytes:
     """The C views of tensor-likes (None: not given) behind one another, as bytes."""
+    if not _fast_looked_for:
+        _load_fast()
     if _fast is not None:
         packed = _fast.views(_validate_only_depth == 0, tensors)
         if packed is not None:

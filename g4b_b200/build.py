@@ -83,6 +83,7 @@ def _compile_views() -> None:
     nvcc_root = Path(_nvcc()).resolve().parents[1]
     libs = Path(torch.__file__).parent / "lib"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DG4B_BUILT_FOR="{torch.__version__} {sys.version.split()[0]} {sys.implementation.cache_tag}"',
            *[f"-I{d}" for d in include_paths()], f"-I{sysconfig.get_paths()['include']}", f"-I{nvcc_root / 'include'}",
            str(CSRC / "views.cpp"), "-o", str(VIEWS), f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -151,4 +151,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_views", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__views(void) { return PyModule_Create(&module); }
+// built_for: the torch and the Python whose headers this was compiled with.  A tensor is read through their inlined
+// layouts, so the module is used with no other (_cabi.py compares).
+PyMODINIT_FUNC PyInit__views(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", G4B_BUILT_FOR) != 0) { Py_DECREF(m); return nullptr; }
+  return m;
+}
