@@ -54,6 +54,23 @@ inline bool contiguous_from(const G4bTensor& t, int from) {
   return true;
 }
 
+// Whether rows of a [rows, heads, D] view lie over one another, so that two writers would meet in one element: for some
+// (i, j) other than (0, 0), |i stride0 - j stride1| < D.  For a given j only the two multiples of stride0 next to j stride1
+// come into question.
+inline bool rows_overlap(const G4bTensor& t) {
+  const int64_t D = t.shape[2], a = t.stride[0], b = t.stride[1], n = t.shape[0], h = t.shape[1];
+  if (n == 0 || h == 0 || D == 0) return false;
+  if ((n > 1 && a < D) || (h > 1 && b < D)) return true;
+  if (a >= (h - 1) * b + D || b >= (n - 1) * a + D) return false;      // (row by row, or head by head: the usual ones)
+  for (int64_t j = 1; n > 1 && j < h; ++j) {
+    const int64_t i = j * b / a;
+    if (i >= n) break;                                     // (further heads lie behind the last row)
+    if (i > 0 && j * b - i * a < D) return true;
+    if (i + 1 < n && (i + 1) * a - j * b < D) return true;
+  }
+  return false;
+}
+
 // True while the calling thread is in validate-only mode: a launcher that has finished its
 // argument checks returns G4B_VALIDATED instead of touching the CUDA runtime.
 bool validate_only_mode();  // api.cu

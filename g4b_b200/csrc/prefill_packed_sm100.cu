@@ -1299,6 +1299,7 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
       if (t.shape[i] > 1 && (t.stride[i] <= 0 || (t.stride[i] * dtype_size(t.dtype)) % 16 != 0))
         return fail(G4B_ERR_BAD_STRIDE, "%s: strides must be positive multiples of 16 bytes", nm);
   }
+  if (rows_overlap(a.o)) return fail(G4B_ERR_BAD_STRIDE, "o: rows that are written must not overlap");
   if ((((uintptr_t)a.q.ptr) | ((uintptr_t)a.o.ptr) | ((uintptr_t)a.k_pool.ptr) | ((uintptr_t)a.v_pool.ptr)) & 15)
     return fail(G4B_ERR_BAD_STRIDE, "q, o and the pools must be 16-byte aligned");
   if (a.workspace.stride[0] != 1 && a.workspace.shape[0] > 1) return fail(G4B_ERR_BAD_STRIDE, "workspace must be contiguous");

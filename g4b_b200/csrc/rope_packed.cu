@@ -333,6 +333,8 @@ int launch_rope_norm_append_packed(const G4bRopePackedArgs& a, cudaStream_t st) 
   if (D % 8 != 0 || D < 8 || D > 512) return fail(G4B_ERR_UNSUPPORTED, "head dim must be a multiple of 8, at most 512");
   if (H < 1 || G < 1) return fail(G4B_ERR_BAD_ARG, "at least one query head and one kv head");
   if (given(a.q_out) && (rc = check_rows(a.q_out, "q_out", N, H, D))) return rc;
+  if (rows_overlap(given(a.q_out) ? a.q_out : a.q))
+    return fail(G4B_ERR_BAD_STRIDE, "%s: rows that are written must not overlap", given(a.q_out) ? "q_out" : "q");
   if ((rc = check_rank(a.rope_freqs, "rope_freqs", 1))) return rc;
   if (a.rope_freqs.shape[0] != D / 2) return fail(G4B_ERR_BAD_ARG, "rope_freqs must have D/2 entries");
   if (a.rope_freqs.dtype != G4B_F32) return fail(G4B_ERR_BAD_DTYPE, "rope_freqs must be f32");

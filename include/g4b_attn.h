@@ -401,7 +401,7 @@ int64_t g4b_exchange_buffer_bytes(int world, int64_t rows, int head_dim);
 typedef struct G4bRopePackedArgs {
   G4bTensor q;              /* [N, H, D] view, last stride 1; f32, f16 or bf16 */
   G4bTensor k, v;           /* [N, G, D] views, q's type */
-  G4bTensor q_out;          /* optional [N, H, D] view, any float type */
+  G4bTensor q_out;          /* optional [N, H, D] view, any float type; rows that are written must not overlap */
   G4bTensor rope_freqs;     /* f32 [D/2] */
   G4bTensor positions;      /* optional int32 or int64 [axes, N] view */
   G4bTensor pair_axis;      /* uint8 [D/2]; optional with one axis */
