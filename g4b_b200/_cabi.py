@@ -232,6 +232,14 @@ def _load_fast() -> None:
         _fast = module
 
 
+def pack_tail(packer: struct.Struct, *values) -> bytes:
+    """The plain numbers at the end of an argument struct; ValueError for what does not fit their 32 bits."""
+    try:
+        return packer.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"argument out of range: {e}") from None
+
+
 def call(name: str, args_type, tensors: tuple, tail: bytes, stream) -> None:
     """Entry point ``name`` on an argument struct that is the views of ``tensors`` (None: not given) and ``tail``."""
     lib = _lib if _lib is not None else load()

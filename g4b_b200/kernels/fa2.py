@@ -216,5 +216,5 @@ def flash_attention_packed(q, k_pool, v_pool, o, q_starts, time_dim_sizes, *, bl
     allocates once; calls that may overlap on the GPU need one each.  Returns None."""
     _cabi.call("g4b_flash_attention_packed", _cabi.G4bPackedAttnArgs,
                (q, o, k_pool, v_pool, q_starts, time_dim_sizes, block_tables, workspace),
-               _PACKED_TAIL.pack(page_size, stage, sliding_window or 0, scale), stream)
+               _cabi.pack_tail(_PACKED_TAIL, int(page_size), int(stage), int(sliding_window or 0), float(scale)), stream)
     return None

@@ -137,7 +137,7 @@ def rope_norm_append_packed(
     pages.  No counterpart in the reference."""
     tensors = (q, k, v, q_out, rope_freqs, positions, pair_axis, q_starts, time_dim_sizes, q_rmsnorm_w, k_rmsnorm_w, k_pool, v_pool,
                block_tables)
-    tail = _PACKED_TAIL.pack(rmsnorm_eps, page_size, 1 if norm_qk else 0, 1 if norm_v else 0)
+    tail = _cabi.pack_tail(_PACKED_TAIL, float(rmsnorm_eps), int(page_size), 1 if norm_qk else 0, 1 if norm_v else 0)
     if positions is None or len(positions.shape) != 1:
         _cabi.call("g4b_rope_norm_append_packed", _cabi.G4bRopePackedArgs, tensors, tail, stream)
         return None
