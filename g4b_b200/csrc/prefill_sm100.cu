@@ -1062,6 +1062,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         ptx::tc_wait_st();
         ptx::tc_fence_before();
         arrive_issuer(bar_pa);
+        // (PV(j-1) ended long ago; asked here, the answer arrives under the exponentials)
+        const bool pv_seen = j == 0 || ptx::mbar_try_wait(bar_pv, (t - 1) & 1);
         const float neg_m = -m_used;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -1072,13 +1074,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         }
         ptx::tmem_st16(trow + s_col + half * 32 + 16, pk + 16);
         l_run += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        // keep the PV-done phase bookkeeping in step; before P(j) is handed over, since a warp held up behind that could
+        // find PV(j) done too and its one-bit phase as it was
+        if (!__all_sync(0xffffffffu, pv_seen || ptx::mbar_wait(bar_pv, (t - 1) & 1))) {
+          record(p.status, kErrPvDone); ok = false; break;
+        }
         ptx::tc_wait_st();
         ptx::tc_fence_before();
         arrive_issuer(bar_pb);
-        // keep the PV-done phase bookkeeping in step (no stall: PV(j-1) ended long ago)
-        if (j > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(bar_pv, (t - 1) & 1))) {
-          record(p.status, kErrPvDone); ok = false;
-        }
         continue;
       }
 
