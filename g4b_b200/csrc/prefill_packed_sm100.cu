@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(256) plan_kernel(const __grid_constant__ Packe
   if (p.may_split) {
     // Shares pay where the longest item alone takes longer than its worker's fair part of everything (and is
     // worth cutting at all).  Both sides: chunks of 1 to 512 rows behind contexts of 777 to 30000 tokens, 8 / 2 heads,
-    // longest item 4 times the fair part: 573 us whole, 175 in shares, in kernels alike but for that; sixteen prompts
+    // longest item 4 times the fair part: 573 us whole, 175 in shares (123 to 146 now), in kernels alike but for that; sixteen prompts
     // of 1 to 2000 rows, longest item half the fair part: 52 us whole, 64 in shares.  Every warp comes to the same answer.
     longest = __reduce_max_sync(0xffffffffu, longest);
 #pragma unroll
@@ -608,7 +608,7 @@ packed_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
       // K chunk = this CTA's 64 keys of the tile x kD (slabs of [64 rows x 64 d]); V chunk = all 128 keys x
       // this CTA's half of the head dim, group by group of rows (a group: slabs of [v_rows x 64 d]), since a step of
       // the product takes 16 keys and does not care where the next 16 lie: one box a group, where K needs one a group and
-      // slab (sixteen prompts over pages of 16: 52.8 -> 51.2 us).  Lane i fetches the i-th group of rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
+      // slab (sixteen prompts over pages of 16: 56.3 -> 55.2 us).  Lane i fetches the i-th group of rows.  Every CTA accounts for its own bytes on CTA 0's barrier.
       auto load_k = [&](int j) {
         const int key0 = (it.tile_lo + j) * kBN + 64 * (int)rank + lane * p.k_rows;
         const int boxes = 64 / p.k_rows;
@@ -1381,7 +1381,9 @@ int launch_prefill_packed(const G4bPackedAttnArgs& a, cudaStream_t st) {
   if (workers > kMaxWorkers) workers = kMaxWorkers;
   if (workers < 1) workers = 1;
   // Shares pay only where items are few (with six a worker the list of whole ones is balanced) and contexts
-  // can be long; what the contexts really are is looked at on the device.  Nor without any of that a third launch.
+  // can be long; what the contexts really are is looked at on the device.  Nor without any of that a third launch.  The bound
+  // is loose: a small step over a manager's wide table has the third launch too, which then finds nothing to join (three
+  // prompts of 62 rows: 13.2 us with a table of three pages, 15.7 us with one of 2048 columns).
   p.may_split = (N / (2 * p.tpt)) * G < 6 * workers && (int64_t)p.max_pages * a.page_size > 8 * kBN;
   if (!p.may_split && workers > max_items * G) workers = max_items * G;
   p.workers = (int)workers;

@@ -16,8 +16,11 @@
 // four consecutive rotation pairs (i, i + D/2) per pass, so a warp holds 32 / kLanes rows at a
 // time; loads of four such sets go out before any is processed.
 //
-// Measured (f32 in, 16 bits out, graph replay): 32768 tokens 94.8 us = 6370 GB/s, 0.97 of the copy; 4417 tokens of three
-// axes 13.3 us.  What bounds it is the issue rate (2.4 of 4 instructions a cycle) next to HBM, as in rope_append.cu.
+// Measured (f32 in, 16 bits out, 8 + 2 + 2 heads of 256, three sets of inputs in turn; 97 to 104 us by the way the passes are
+// timed): 32768 tokens 97.5 us = 6190 GB/s, 0.95 of the copy; 4417 tokens of three axes 20.1 us (launches alone 18.2; 13.1
+// with one set, which stays in L2).  32 / 28 / 24 warps an SM: 97.5 / 100.8 / 106.6 and 20.1 / 24.1 / 24.3 us; 4300 tokens at head dim
+// 128, where 32 warps leave 64 registers and 48 to 72 bytes of spills, 13.9 / 15.4 / 15.8 us.  What bounds it is the issue rate (2.4 of 4
+// instructions a cycle) next to HBM, as in rope_append.cu.
 #include "common.cuh"
 
 namespace g4b {
@@ -261,8 +264,9 @@ __global__ void __launch_bounds__(32, kIters == 1 ? 32 : 16) rope_packed_kernel(
         // turns, reduced to [-1/2, 1/2] before they become 32 bits
         double turns = (double)pos * ((double)p.freqs[(d + i) * p.freq_s] * 0.15915494309189533577);
         turns -= rint(turns);
-        // the reduced angle is in [-pi, pi], where the fast functions are off by at most 2^-21: less than 1/500 of
-        // what a 16-bit output is rounded by (32768 tokens: 98.8 -> 94.8 us, 4417 of three axes: 15.2 -> 13.3 us)
+        // the reduced angle is in [-pi, pi], where the fast functions are off by at most 2^-21.  An output is off by that
+        // much of its pair's magnitude: 1/500 of a 16-bit rounding where it is about as large as the pair; more of its own rounding
+        // where the two products cancel, as any 32-bit rotation's is (32768 tokens: 98.8 -> 97.5 us, 4417 of three axes: 20.8 -> 20.1)
         if constexpr (kOut != 0) __sincosf(6.2831853f * (float)turns, &s4[i], &c4[i]);
         else sincospif(2.f * (float)turns, &s4[i], &c4[i]);
       }
@@ -415,7 +419,9 @@ int launch_rope_norm_append_packed(const G4bRopePackedArgs& a, cudaStream_t st) 
   p.status = device_status_ptr();
   if (p.status == nullptr) return G4B_ERR_CUDA;
   // Few rows (decode): the rows a warp holds at a time, for parallelism.  Many (prefill): a warp
-  // takes all heads of a token and computes the token's sines and cosines once.
+  // takes all heads of a token and computes the token's sines and cosines once.  All heads / the former: 12 heads of 256, 512
+  // tokens 7.3 / 6.1 us, 1024 tokens 7.7 / 9.4, 1365 tokens 8.6 / 11.9, 4096 tokens 17.8 / 32.5; 12 heads of 128, 512 tokens 5.9 / 4.4,
+  // 1365 tokens 6.5 / 7.5.
   p.heads_per_warp = N * p.n_heads >= 16384 ? p.n_heads : (D == 128 ? 2 : 1);
   p.n_slots = (uint32_t)((p.n_heads + p.heads_per_warp - 1) / p.heads_per_warp);
   const int64_t blocks = N * (int64_t)p.n_slots;
