@@ -387,8 +387,9 @@ int launch_rope_norm_append_packed(const G4bRopePackedArgs& a, cudaStream_t st) 
   if (a.k_pool.dtype != a.v_pool.dtype || a.k_pool.shape[0] != a.v_pool.shape[0])
     return fail(G4B_ERR_BAD_ARG, "k_pool and v_pool must have one dtype and shape");
   if (a.page_size <= 0 || (a.page_size & (a.page_size - 1)) != 0) return fail(G4B_ERR_BAD_ARG, "page_size must be a power of two");
-  if (a.k_pool.shape[0] > 0x7fffffffLL || a.block_tables.shape[1] > 0x7fffffffLL || B > 0x7ffffffeLL)
-    return fail(G4B_ERR_TOO_LARGE, "pages and slots are counted in 31 bits");
+  if (a.k_pool.shape[0] > 0x7fffffffLL || a.block_tables.shape[1] > 0x7fffffffLL)
+    return fail(G4B_ERR_TOO_LARGE, "pages are counted in 31 bits");
+  if (B > 1 << 24) return fail(G4B_ERR_TOO_LARGE, "at most %d slots", 1 << 24);      // (every warp looks at all of their starts)
   if ((a.norm_qk != 0 || a.norm_v != 0) && !(a.rmsnorm_eps > -INFINITY && a.rmsnorm_eps < INFINITY))
     return fail(G4B_ERR_BAD_ARG, "rmsnorm_eps must be finite");
   G4B_STOP_IF_VALIDATE_ONLY();

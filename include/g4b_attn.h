@@ -396,7 +396,7 @@ int64_t g4b_exchange_buffer_bytes(int world, int64_t rows, int head_dim);
  * the cache.  q goes to q_out, or back into q; k and v go to the pools.  A row whose place is
  * outside the block table or whose table entry is outside the pool is not appended (0x101 / 0x102
  * in the device status word); a pair_axis entry past the axes is taken as 0 (0x106).  q_starts that
- * decrease or leave [0, N]: nothing is written (0x107).
+ * decrease or leave [0, N]: nothing is written (0x107).  At most 2^24 slots.
  */
 typedef struct G4bRopePackedArgs {
   G4bTensor q;              /* [N, H, D] view, last stride 1; f32, f16 or bf16 */
